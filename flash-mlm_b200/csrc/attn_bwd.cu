@@ -1,0 +1,176 @@
+// C-ABI entry point of the attention backward pass: argument checks, tensor
+// maps and the three launches (row statistics, Q pass, KV pass).
+#include <cmath>
+#include <type_traits>
+
+#include "common.h"
+#include "tma_map.h"
+
+#include "attn_bwd.cuh"
+
+namespace fmlm {
+namespace {
+
+constexpr unsigned long long kTimeoutNs = 2000000000ull;  // 2 s per wait
+constexpr size_t kCounterBytes = 256;
+
+template <int D, bool KV, bool BF16>
+int launch_pass(const CUtensorMap* m, const BwdParams& p, cudaStream_t s) {
+  using C = BwdCfg<D, KV>;
+  auto kern = attn_bwd_kernel<D, KV, BF16>;
+  // One CTA per SM: a second one would block in tcgen05.alloc.
+  const int smem = std::max(C::SMEM_BYTES, 116 * 1024);
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return set_error(FMLM_ERR_CUDA, "device ordinal %d out of range", dev);
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return set_error(FMLM_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  kern<<<std::min(p.num_items, device_sm_count()), C::THREADS, smem, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+  return check_launch("attn_bwd_kernel");
+}
+
+template <int D, bool KV, bool BF16>
+int run_pass(const fmlm_attn_bwd_args* a, BwdParams p, cudaStream_t s) {
+  using C = BwdCfg<D, KV>;
+  const long long items = (long long)(KV ? p.HK : p.H) * (p.slots + (KV ? p.cslots : 0)) * C::NDH;
+  if (items > 0x7fff0000LL) return set_error(FMLM_ERR_INVALID, "problem too large");
+  if (items == 0) return FMLM_OK;
+  p.num_items = (int)items;
+  p.counter += KV ? 1 : 0;
+  const fmlm_view4 empty = {nullptr, 0, 0, 0, 0, 0, 0};
+  const bool ctx = p.C > 0 && p.Tc > 0;
+  const int qrows = KV ? C::BN : C::BM, krows = KV ? C::BM : C::BN;
+  CUtensorMap m[6];
+  int rc;
+  if ((rc = encode_view(&m[0], a->q, D, qrows, a->dtype, a->q.data, "q"))) return rc;
+  if ((rc = encode_view(&m[1], a->dout, D, qrows, a->dtype, a->q.data, "dout"))) return rc;
+  if ((rc = encode_view(&m[2], a->k, D, krows, a->dtype, a->q.data, "k"))) return rc;
+  if ((rc = encode_view(&m[3], a->v, D, krows, a->dtype, a->q.data, "v"))) return rc;
+  if ((rc = encode_view(&m[4], ctx ? a->k_context : empty, D, krows, a->dtype, a->q.data, "k_context"))) return rc;
+  if ((rc = encode_view(&m[5], ctx ? a->v_context : empty, D, krows, a->dtype, a->q.data, "v_context"))) return rc;
+  return launch_pass<D, KV, BF16>(m, p, s);
+}
+
+template <int D, bool BF16>
+int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cudaStream_t s) {
+  const long long vecs = rows * (D / 8);
+  const long long blocks = (vecs + 255) / 256;
+  if (blocks > 0x7fffffffLL) return set_error(FMLM_ERR_INVALID, "problem too large");
+  attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
+      reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, rows,
+      const_cast<float2*>(p.stats), p.counter);
+  int rc = check_launch("attn_bwd_stats_kernel");
+  if (!rc && a->dq) rc = run_pass<D, false, BF16>(a, p, s);
+  if (!rc && a->dk) rc = run_pass<D, true, BF16>(a, p, s);
+  return rc;
+}
+
+template <bool BF16>
+int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cudaStream_t s) {
+  switch (a->head_dim) {
+    case 16: return run_bwd<16, BF16>(a, p, rows, s);
+    case 32: return run_bwd<32, BF16>(a, p, rows, s);
+    case 64: return run_bwd<64, BF16>(a, p, rows, s);
+    case 128: return run_bwd<128, BF16>(a, p, rows, s);
+    case 256: return run_bwd<256, BF16>(a, p, rows, s);
+    default: return set_error(FMLM_ERR_UNSUPPORTED, "HEAD_DIM must be one of {16, 32, 64, 128, 256}");
+  }
+}
+
+int check_view(const fmlm_view4& v, const char* name, int64_t rows, int64_t heads, int64_t batch) {
+  if (!v.data) return set_error(FMLM_ERR_INVALID, "%s is required", name);
+  if (v.rows != rows || v.heads != heads || v.batch != batch)
+    return set_error(FMLM_ERR_INVALID, "%s: the view must be [%lld][%lld][%lld][head_dim]", name, (long long)batch,
+                     (long long)heads, (long long)rows);
+  return FMLM_OK;
+}
+
+}  // namespace
+}  // namespace fmlm
+
+using namespace fmlm;
+
+extern "C" size_t fmlm_attn_bwd_workspace_bytes(int64_t rows) {
+  return kCounterBytes + (size_t)(rows > 0 ? rows : 0) * sizeof(float2);
+}
+
+extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
+  if (!a) return set_error(FMLM_ERR_INVALID, "null args");
+  if (a->dtype != FMLM_DTYPE_F16 && a->dtype != FMLM_DTYPE_BF16) return set_error(FMLM_ERR_INVALID, "dtype must be f16 or bf16");
+  const int D = a->head_dim;
+  const bool packed = a->layout == FMLM_BWD_PACKED;
+  if (a->layout < FMLM_BWD_DENSE || a->layout > FMLM_BWD_PACKED) return set_error(FMLM_ERR_INVALID, "bad layout");
+  if (a->batch < 1 || a->num_heads < 1 || a->kv_heads < 1 || a->num_heads % a->kv_heads != 0)
+    return set_error(FMLM_ERR_INVALID, "batch, num_heads, kv_heads must be >= 1 and num_heads a multiple of kv_heads");
+  if (!packed && (a->seq_len < 1 || a->seq_len > 0x3fffff00)) return set_error(FMLM_ERR_INVALID, "seq_len must be in [1, 2^30)");
+  if (packed && (a->total_q_len < 1 || a->total_q_len > 0x3fffff00LL))
+    return set_error(FMLM_ERR_INVALID, "total_q_len must be in [1, 2^30)");
+  if (!packed && (a->causal_query_seq_attn || a->context_entries))
+    return set_error(FMLM_ERR_INVALID, "causal_query_seq_attn and a context need the packed layout");
+  if (a->layout != FMLM_BWD_DENSE && !a->cu_seqlens_q) return set_error(FMLM_ERR_INVALID, "cu_seqlens_q is required");
+  if (a->context_entries != 0 && a->context_entries != 1 && a->context_entries != a->batch)
+    return set_error(FMLM_ERR_INVALID, "context_entries must be 0, 1 or batch");
+  if (!a->error_word) return set_error(FMLM_ERR_INVALID, "error_word is required");
+  const int64_t qr = packed ? a->total_q_len : a->seq_len, qb = packed ? 1 : a->batch;
+  int rc;
+  if ((rc = check_view(a->q, "q", qr, a->num_heads, qb))) return rc;
+  if ((rc = check_view(a->dout, "dout", qr, a->num_heads, qb))) return rc;
+  if ((rc = check_view(a->k, "k", qr, a->kv_heads, qb))) return rc;
+  if ((rc = check_view(a->v, "v", qr, a->kv_heads, qb))) return rc;
+  if (a->dout.row_stride != D || (a->num_heads > 1 && a->dout.head_stride != qr * D) ||
+      (qb > 1 && a->dout.batch_stride != a->num_heads * qr * D))
+    return set_error(FMLM_ERR_INVALID, "dout must be contiguous");
+  const bool ctx = a->context_entries > 0 && a->total_context_len > 0;
+  if (ctx) {
+    if (a->total_context_len > 0x3fffff00LL) return set_error(FMLM_ERR_INVALID, "total_context_len must be < 2^30");
+    if (!a->cu_seqlens_context || (a->dk && (!a->dk_context || !a->dv_context)))
+      return set_error(FMLM_ERR_INVALID, "a context needs cu_seqlens_context, and dk_context and dv_context with dk");
+    if ((rc = check_view(a->k_context, "k_context", a->total_context_len, a->kv_heads, 1))) return rc;
+    if ((rc = check_view(a->v_context, "v_context", a->total_context_len, a->kv_heads, 1))) return rc;
+    if (!aligned16(a->dk_context) || !aligned16(a->dv_context))
+      return set_error(FMLM_ERR_INVALID, "dk_context and dv_context must be 16-byte aligned");
+  }
+  if ((a->dk == nullptr) != (a->dv == nullptr) || (!a->dq && !a->dk))
+    return set_error(FMLM_ERR_INVALID, "give dq, or dk and dv, or all three");
+  if (!a->out || !a->lse || !aligned16(a->out) || !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv))
+    return set_error(FMLM_ERR_INVALID, "out and lse are required; out, dq, dk, dv must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->dout.data) & 15u) != 0) return set_error(FMLM_ERR_INVALID, "dout must be 16-byte aligned");
+  const int64_t rows = qb * a->num_heads * qr;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < fmlm_attn_bwd_workspace_bytes(rows))
+    return set_error(FMLM_ERR_INVALID, "workspace too small (%zu bytes needed)", fmlm_attn_bwd_workspace_bytes(rows));
+
+  BwdParams p{};
+  p.layout = a->layout;
+  p.B = a->batch;
+  p.H = a->num_heads;
+  p.HK = a->kv_heads;
+  p.G = a->num_heads / a->kv_heads;
+  p.N = a->seq_len;
+  p.T = packed ? (int)a->total_q_len : 0;
+  p.C = ctx ? a->context_entries : 0;
+  p.Tc = ctx ? (int)a->total_context_len : 0;
+  p.causal = a->causal_query_seq_attn;
+  const long long slots = packed ? p.T / 128 + p.B : (long long)p.B * ((p.N + 127) / 128);
+  if (slots > 0x3fffffffLL) return set_error(FMLM_ERR_INVALID, "problem too large");
+  p.slots = (int)slots;
+  p.cslots = p.C > 0 ? p.Tc / 128 + p.C : 0;
+  p.cu_q = a->cu_seqlens_q;
+  p.cu_c = a->cu_seqlens_context;
+  p.counter = reinterpret_cast<int*>(a->workspace);
+  p.stats = reinterpret_cast<const float2*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
+  p.dq = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  p.dkc = a->dk_context;
+  p.dvc = a->dv_context;
+  p.scale = a->scale;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.err = a->error_word;
+  p.timeout_ns = kTimeoutNs;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->dtype == FMLM_DTYPE_BF16 ? dispatch_bwd<true>(a, p, rows, s) : dispatch_bwd<false>(a, p, rows, s);
+}

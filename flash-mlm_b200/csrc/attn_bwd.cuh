@@ -1,0 +1,673 @@
+// Backward pass of the bidirectional attention for sm_100a (B200).
+//
+// With S = scale * q k^T, P = exp(S - lse) (lse saved by the forward pass),
+// dP = dO v^T and delta = rowsum(dO * O):
+//   dS = P * (dP - delta),  dV = P^T dO,  dQ = scale * dS k,  dK = scale * dS^T q.
+// The probabilities are recomputed tile by tile; nothing of size Nq x Nkv is
+// stored.  Two passes over the score tiles, each owning its outputs, so no
+// floating-point atomics are needed and the same inputs give the same bits:
+//   KV pass  a work item owns 128 keys of one key head; the queries that see
+//            them (of every query head of the group) stream past; dK and dV
+//            accumulate in TMEM.
+//   Q pass   a work item owns 128 queries; their keys stream past (context,
+//            then main); dQ accumulates in TMEM.
+// Both are one kernel: stationary tiles A1, A2 (128 rows), streamed tiles B1, B2:
+//   S = A1 B1^T,  dP = A2 B2^T            (KV: A = K, V; B = Q, dO.  Q: A = Q, dO; B = K, V)
+//   acc2 += dS B1,  KV: acc1 += P B2      (P, dS: 16-bit, A operand from TMEM)
+// In the KV pass S and dP are the transposed scores, so P^T and dS^T leave the
+// registers in the layout in which the tensor cores read A from TMEM, as in
+// the Q pass; P and dS never touch shared memory.
+//
+// Roles of a persistent CTA (one per SM): warps 0-7 do the element-wise work
+// (warp w: TMEM lanes 32 (w % 4) .., column half w / 4 of every score tile),
+// warp 8 loads tiles by TMA and decodes work items, warp 9 issues the MMAs.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace fmlm {
+
+struct BwdParams {
+  int layout;  // FMLM_BWD_*
+  int B, H, HK, G, N;
+  int T, Tc;   // packed rows per head; context rows per head
+  int C;       // context entries (0: none)
+  int causal;
+  int slots, cslots;  // tile slots of a head over the sequences / context entries
+  int num_items;
+  const int* cu_q;
+  const int* cu_c;
+  const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta * 2^-kPExp}
+  int* counter;
+  void *dq, *dk, *dv, *dkc, *dvc;
+  float scale, scale_log2;
+  int* err;
+  unsigned long long timeout_ns;
+};
+
+template <int D_, bool KV_>
+struct BwdCfg {
+  static constexpr int D = D_;
+  static constexpr bool KV = KV_;
+  static constexpr int BM = 128;
+  static constexpr int BN = D == 256 ? 64 : 128;  // streamed rows per tile (D = 256: what shared memory holds)
+  // D = 256: dK and dV of 128 keys (512 fp32 columns) would fill TMEM, so a KV
+  // item makes one 128-column half of both and the scores are computed twice.
+  static constexpr int DV = (KV && D == 256) ? 128 : D;
+  static constexpr int NDH = D / DV;
+  static constexpr int SWB = D * 2 >= 128 ? 128 : D * 2;
+  static constexpr int SLAB_COLS = SWB / 2;
+  static constexpr int NSLAB = D / SLAB_COLS;
+  static constexpr int A_BYTES = BM * D * 2;
+  static constexpr int B_BYTES = BN * D * 2;
+  static constexpr int ABUF = D <= 64 ? 2 : 1;
+  static constexpr int STAGES = D <= 64 ? 4 : D == 128 ? 2 : 1;
+  static constexpr int EW_WARPS = 8;
+  static constexpr int TMA_WARP = EW_WARPS;
+  static constexpr int MMA_WARP = EW_WARPS + 1;
+  static constexpr int THREADS = 32 * (EW_WARPS + 2);
+  static constexpr int NC = BN / 2;  // score columns per element-wise warp
+  static constexpr int TM_S = 0, TM_DP = BN, TM_ACC1 = 2 * BN, TM_ACC2 = 2 * BN + (KV ? DV : 0);
+  static constexpr int TMEM_USED = TM_ACC2 + DV;
+  static_assert(TMEM_USED <= 512, "TMEM budget");
+  static constexpr int TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
+  static constexpr int STAT_BYTES = KV ? STAGES * BN * 8 : 0;
+  static constexpr int SMEM_TILES = 2 * ABUF * A_BYTES + 2 * STAGES * B_BYTES;
+  static constexpr int RING = 4;
+  static constexpr int ITEM_BYTES = 96;
+  static constexpr int SMEM_BYTES = SMEM_TILES + STAT_BYTES + 512 + RING * ITEM_BYTES + 1024;
+};
+
+// A work item: the stationary tile, the rows it writes and up to two ranges of
+// streamed rows (the KV pass walks its one range once per query head of the group).
+struct BwdItem {
+  int a_map, a_row, a_h, a_b;  // stationary tile: 0 main tensors, 1 context; coordinates
+  int valid, limit;            // rows [0, valid) hold results, [valid, limit) get zeros
+  int dh;                      // D = 256 KV pass: 128-column half
+  int heads, h0, b;            // streamed heads h0 .. h0 + heads - 1, batch coordinate
+  int map0, row0, end0, nt0;   // first range (context when map0 = 1)
+  int row1, end1, nt1;         // second range (main)
+  int stat_h;                  // KV: stats rows of one streamed head
+  long long out_row;           // output row of the tile's row 0 (also its stats row in the Q pass)
+  long long stat0;             // KV: stats row of (head h0, streamed row 0)
+};
+static_assert(sizeof(BwdItem) <= 96, "item ring slot");
+
+// The sequence that owns tile slot v when sequence b's tiles start at slot
+// cu[b] / 128 + b (strictly increasing, and at least ceil(len / 128) apart, so
+// no scan is needed).  A 32-way search by the whole warp.
+__device__ __forceinline__ int find_slot_owner(const int* __restrict__ cu, int n, int v, int lane) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5;
+    const int i = lo + lane * step;
+    const bool le = i < hi && (lane == 0 || ((__ldg(cu + i) >> 7) + i) <= v);
+    const unsigned m = __ballot_sync(0xffffffffu, le);
+    const int top = 31 - __clz(m);
+    lo += top * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+template <class C>
+__device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, int lane) {
+  BwdItem it;
+  constexpr int BN = C::BN;
+  auto tiles = [](int r0, int r1) { return r1 > r0 ? (r1 - r0 + BN - 1) / BN : 0; };
+  it.dh = w % C::NDH;
+  w /= C::NDH;
+  // KV: the context's slots first (a shared context streams the whole batch past: the longest items)
+  const int per_head = p.slots + (C::KV ? p.cslots : 0);
+  const int h = w / per_head;
+  int v = w % per_head;
+  const bool ctx = C::KV && v < p.cslots;
+  if (C::KV && !ctx) v -= p.cslots;
+  const bool packed = p.layout == FMLM_BWD_PACKED;
+  it.map0 = 0; it.row1 = it.end1 = it.nt1 = 0;
+  it.a_map = ctx ? 1 : 0;
+  it.a_h = h;
+  it.a_b = it.b = 0;
+  it.heads = C::KV ? p.G : 1;
+  it.h0 = C::KV ? h * p.G : h / p.G;
+  it.stat_h = 0;
+  it.stat0 = 0;
+  if (ctx) {
+    const int c = find_slot_owner(p.cu_c, p.C, v, lane);
+    const int c0 = min(max(__ldg(p.cu_c + c), 0), p.Tc), c1 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
+    const int t = v - ((c0 >> 7) + c);
+    it.a_row = c0 + t * 128;
+    it.valid = it.limit = min(max(c1 - it.a_row, 0), t >= 0 ? 128 : 0);
+    it.out_row = (long long)h * p.Tc + it.a_row;
+    const int e = p.C == 1 ? p.B : c + 1;
+    it.row0 = min(max(__ldg(p.cu_q + (p.C == 1 ? 0 : c)), 0), p.T);
+    it.end0 = min(max(__ldg(p.cu_q + e), 0), p.T);
+    it.stat_h = p.T;
+  } else if (packed) {
+    const int b = find_slot_owner(p.cu_q, p.B, v, lane);
+    const int s0 = min(max(__ldg(p.cu_q + b), 0), p.T), s1 = min(max(__ldg(p.cu_q + b + 1), 0), p.T);
+    const int t = v - ((s0 >> 7) + b);
+    it.a_row = s0 + t * 128;
+    it.valid = it.limit = min(max(s1 - it.a_row, 0), t >= 0 ? 128 : 0);
+    it.out_row = (long long)h * p.T + it.a_row;
+    it.stat_h = p.T;
+    it.row0 = s0;
+    it.end0 = s1;
+    if (C::KV && p.causal) it.end0 = min(max(__ldg(p.cu_q + p.B), 0), p.T);
+    if (!C::KV) {
+      if (p.causal) it.row0 = 0;
+      if (p.C > 0) {  // context first, then main
+        const int c = p.C == 1 ? 0 : b;
+        it.row1 = it.row0; it.end1 = it.end0;
+        it.nt1 = tiles(it.row1, it.end1);
+        it.map0 = 1;
+        it.row0 = min(max(__ldg(p.cu_c + c), 0), p.Tc);
+        it.end0 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
+      }
+    }
+  } else {
+    const int per_seq = (p.N + 127) / 128;
+    const int b = v / per_seq, t = v % per_seq;
+    int L = p.N;
+    if (p.layout == FMLM_BWD_PADDED) L = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
+    it.a_row = t * 128;
+    it.a_b = it.b = b;
+    it.valid = min(max(L - it.a_row, 0), 128);
+    it.limit = min(p.N - it.a_row, 128);
+    it.out_row = ((long long)b * (C::KV ? p.HK : p.H) + h) * p.N + it.a_row;
+    it.row0 = 0;
+    it.end0 = L;
+    it.stat_h = p.N;
+  }
+  if (C::KV) it.stat0 = ((long long)(packed ? 0 : it.b) * p.H + it.h0) * it.stat_h;
+  it.nt0 = tiles(it.row0, it.end0);
+  if (it.valid == 0) it.nt0 = it.nt1 = 0;
+  return it;
+}
+
+struct __align__(8) BwdBarriers {
+  uint64_t a_full[2], a_empty[2];
+  uint64_t b1_full[4], b2_full[4], b1_empty[4], b2_empty[4];
+  uint64_t s_full, dp_full;  // MMA -> element-wise: S / dP complete
+  uint64_t p_full, ds_full;  // element-wise -> MMA: P written (Q pass: S read) / dS written
+  uint64_t acc_full, acc_empty;
+  uint64_t item_full[4], item_empty[4];
+  int item_idx[4];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(BwdBarriers) <= 512, "barrier block is reserved 512 bytes");
+
+// float16 holds P scaled by 2^12 (P <= 1): small probabilities of long rows
+// stay clear of its subnormals.  bfloat16 has the exponent range as it is.
+template <bool BF16>
+struct BwdScale {
+  static constexpr float kPExp = BF16 ? 0.f : 12.f;
+  static constexpr float kInv = BF16 ? 1.f : 1.f / 4096.f;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+
+template <int D, bool KV, bool BF16>
+__global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                    const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc,
+                    const BwdParams p) {
+  using C = BwdCfg<D, KV>;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  constexpr int BN = C::BN, SWB = C::SWB, STAGES = C::STAGES, NC = C::NC;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;                            // [ABUF][A1, A2]
+  uint8_t* sB = sA + 2 * C::ABUF * C::A_BYTES;   // [STAGES][B1, B2]
+  float* sStat = reinterpret_cast<float*>(sB + 2 * STAGES * C::B_BYTES);  // KV: [STAGES][2][BN]
+  BwdBarriers* bar = reinterpret_cast<BwdBarriers*>(reinterpret_cast<uint8_t*>(sStat) + C::STAT_BYTES);
+  BwdItem* ring_items = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(bar) + 512);
+  volatile int* abort_flag = &bar->abort_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->a_full[i], 1);
+      mbar_init(&bar->a_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&bar->b1_full[i], KV ? 2 : 1);  // KV: the tile, and its rows' stats
+      mbar_init(&bar->b2_full[i], 1);
+      mbar_init(&bar->b1_empty[i], 1);
+      mbar_init(&bar->b2_empty[i], 1);
+      mbar_init(&bar->item_full[i], 1);
+      mbar_init(&bar->item_empty[i], C::EW_WARPS + 1);
+    }
+    mbar_init(&bar->s_full, 1);
+    mbar_init(&bar->dp_full, 1);
+    mbar_init(&bar->p_full, C::EW_WARPS);
+    mbar_init(&bar->ds_full, C::EW_WARPS);
+    mbar_init(&bar->acc_full, 1);
+    mbar_init(&bar->acc_empty, C::EW_WARPS);
+    bar->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == C::MMA_WARP) {
+    tmem_alloc(&bar->tmem_base, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == C::TMA_WARP && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_do);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = bar->tmem_base;
+  const uint64_t tmo = p.timeout_ns;
+  const int num_items = p.num_items;
+  bool failed = false;
+
+  auto fail = [&]() {
+    failed = true;
+    *abort_flag = 1;
+    atomicExch(p.err, 1);
+  };
+  // Whole-warp wait; false once anything in the CTA has given up.
+  auto wait = [&](uint64_t* b, uint32_t ph) -> bool {
+    if (!mbar_wait(b, ph, abort_flag, tmo)) fail();
+    failed = __any_sync(0xffffffffu, failed);
+    return !failed;
+  };
+  auto take_item = [&](uint32_t ring, BwdItem& it) -> bool {
+    if (failed || !wait(&bar->item_full[ring & 3], (ring >> 2) & 1u)) return false;
+    const int w = *reinterpret_cast<volatile int*>(&bar->item_idx[ring & 3]);
+    if (w < num_items) it = ring_items[ring & 3];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar->item_empty[ring & 3]);
+    return w < num_items;
+  };
+
+  if (warp == C::TMA_WARP) {
+    // ------------------------------------------------------------ producer
+    uint32_t fill = 0, aload = 0;
+    int w = blockIdx.x;
+    auto load_tile = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* b, int rows, int row, int h, int bb) {
+      for (int s = 0; s < C::NSLAB; ++s) tma_load_4d(dst + s * (rows * SWB), m, b, s * C::SLAB_COLS, row, h, bb);
+    };
+    for (uint32_t ring = 0;; ++ring) {
+      BwdItem it;
+      if (w < num_items) it = decode_bwd_item<C>(p, w, lane);
+      if (!wait(&bar->item_empty[ring & 3], ((ring >> 2) & 1u) ^ 1u)) break;
+      if (lane == 0) {
+        if (w < num_items) ring_items[ring & 3] = it;
+        bar->item_idx[ring & 3] = w;
+        mbar_arrive(&bar->item_full[ring & 3]);
+      }
+      __syncwarp();
+      if (w >= num_items) break;
+      const int n = it.heads * it.nt0 + it.nt1;
+      if (n > 0) {
+        const int ab = aload % C::ABUF;
+        if (!wait(&bar->a_empty[ab], ((aload / C::ABUF) & 1u) ^ 1u)) break;
+        if (lane == 0) {
+          const CUtensorMap* m1 = KV ? (it.a_map ? &tm_kc : &tm_k) : &tm_q;
+          const CUtensorMap* m2 = KV ? (it.a_map ? &tm_vc : &tm_v) : &tm_do;
+          uint8_t* dst = sA + ab * 2 * C::A_BYTES;
+          mbar_arrive_expect_tx(&bar->a_full[ab], 2 * C::A_BYTES);
+          load_tile(dst, m1, &bar->a_full[ab], C::BM, it.a_row, it.a_h, it.a_b);
+          load_tile(dst + C::A_BYTES, m2, &bar->a_full[ab], C::BM, it.a_row, it.a_h, it.a_b);
+        }
+        __syncwarp();
+        ++aload;
+        int g = 0, t = 0;  // streamed head, tile within it (Q pass: tile over both ranges)
+        for (int i = 0; i < n && !failed; ++i, ++fill) {
+          const int st = fill % STAGES;
+          const uint32_t ph = (fill / STAGES) & 1u;
+          const bool second = !KV && t >= it.nt0;
+          const int row = second ? it.row1 + (t - it.nt0) * BN : it.row0 + t * BN;
+          const int end = second ? it.end1 : it.end0;
+          const int h = it.h0 + g;
+          const bool cmap = !KV && it.map0 == 1 && !second;
+          uint8_t* d1 = sB + st * 2 * C::B_BYTES;
+          if (!wait(&bar->b1_empty[st], ph ^ 1u)) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bar->b1_full[st], C::B_BYTES);
+            load_tile(d1, KV ? &tm_q : cmap ? &tm_kc : &tm_k, &bar->b1_full[st], BN, row, h, it.b);
+          }
+          __syncwarp();
+          if (!wait(&bar->b2_empty[st], ph ^ 1u)) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bar->b2_full[st], C::B_BYTES);
+            load_tile(d1 + C::B_BYTES, KV ? &tm_do : cmap ? &tm_vc : &tm_v, &bar->b2_full[st], BN, row, h, it.b);
+          }
+          __syncwarp();
+          if constexpr (KV) {
+            // The streamed rows' statistics; rows past the range get P = 0.
+            const float2* src = p.stats + it.stat0 + (long long)g * it.stat_h;
+            float* ss = sStat + st * 2 * BN;
+#pragma unroll
+            for (int c = lane; c < BN; c += 32) {
+              const float2 x = row + c < end ? __ldg(src + row + c) : make_float2(-INFINITY, 0.f);
+              ss[c] = x.x;
+              ss[BN + c] = x.y;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->b1_full[st]);
+          }
+          if (++t == it.nt0 && KV) { t = 0; ++g; }
+        }
+        if (failed) break;
+      }
+      int next = 0;
+      if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
+      w = __shfl_sync(0xffffffffu, next, 0);
+    }
+  } else if (warp == C::MMA_WARP) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t fmt = BF16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, C::BM, BN);
+    constexpr uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, C::BM, C::DV);
+    constexpr uint32_t layout = swizzle_code(SWB);
+    const uint32_t sA0 = smem_u32(sA), sB0 = smem_u32(sB);
+    const bool leader = elect_one();
+    uint32_t fill = 0, aload = 0, p_ph = 0, ds_ph = 0, acc_ph = 1;
+    // scores: D[128, BN] = A[128, D] B[BN, D]^T
+    auto issue_scores = [&](uint32_t d, uint32_t a_base, uint32_t b_base) {
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t slab = (kk * 32) / SWB, inrow = (kk * 32) % SWB;
+          umma_ss(d, make_smem_desc(a_base + slab * (C::BM * SWB) + inrow, 16, 8 * SWB, layout),
+                  make_smem_desc(b_base + slab * (BN * SWB) + inrow, 16, 8 * SWB, layout), idesc_s, kk > 0 ? 1u : 0u);
+        }
+      }
+    };
+    // accumulators: D[128, DV] += A[128, BN] (16-bit, TMEM) B[BN, DV]; each
+    // column half of A lies at the start of that half of the score tile.
+    auto issue_acc = [&](uint32_t d, uint32_t a_tm, uint32_t b_base, bool acc) {
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk) {
+          constexpr int HK = BN / 32;  // K steps per half
+          const uint32_t a = a_tm + (kk / HK) * (BN / 2) + (kk % HK) * 8;
+          umma_ts(d, a, make_smem_desc(b_base + kk * 16 * SWB, BN * SWB, 8 * SWB, layout), idesc_acc,
+                  (acc || kk > 0) ? 1u : 0u);
+        }
+      }
+    };
+    auto commit = [&](uint64_t* b) {
+      if (leader) umma_commit(b);
+      __syncwarp();
+    };
+    // Rows past the range hold another sequence's rows or padding, NaN perhaps:
+    // P and dS are 0 there, but 0 * NaN is not.
+    auto clear_rows = [&](uint8_t* tile, int valid) {
+      if (valid < BN) {
+        for (int s = 0; s < C::NSLAB; ++s) {
+          uint4* z = reinterpret_cast<uint4*>(tile + s * (BN * SWB) + valid * SWB);
+          for (int i = lane; i < (BN - valid) * SWB / 16; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+    };
+    BwdItem it;
+    for (uint32_t ring = 0; take_item(ring, it); ++ring) {
+      const int n = it.heads * it.nt0 + it.nt1;
+      if (n == 0) continue;
+      const int ab = aload % C::ABUF;
+      if (!wait(&bar->a_full[ab], (aload / C::ABUF) & 1u)) break;
+      ++aload;
+      const uint32_t a1 = sA0 + ab * 2 * C::A_BYTES, a2 = a1 + C::A_BYTES;
+      const uint32_t dh_off = (it.dh * C::DV / C::SLAB_COLS) * (BN * SWB);
+      // valid rows of streamed tile i; tiles are asked for in order, each twice (S, dP)
+      auto valid_rows = [&](int i) {
+        int t = KV ? i % it.nt0 : i;
+        if (!KV && t >= it.nt0) return it.end1 - (it.row1 + (t - it.nt0) * BN);
+        return it.end0 - (it.row0 + t * BN);
+      };
+      auto do_s = [&](int i) -> bool {
+        const uint32_t f = fill + i;
+        const int st = f % STAGES;
+        if (!wait(&bar->b1_full[st], (f / STAGES) & 1u)) return false;
+        clear_rows(sB + st * 2 * C::B_BYTES, valid_rows(i));
+        tc_fence_after();
+        issue_scores(tmem_base + C::TM_S, a1, sB0 + st * 2 * C::B_BYTES);
+        commit(&bar->s_full);
+        return true;
+      };
+      auto do_dp = [&](int i) -> bool {
+        const uint32_t f = fill + i;
+        const int st = f % STAGES;
+        if (!wait(&bar->b2_full[st], (f / STAGES) & 1u)) return false;
+        clear_rows(sB + st * 2 * C::B_BYTES + C::B_BYTES, valid_rows(i));
+        tc_fence_after();
+        issue_scores(tmem_base + C::TM_DP, a2, sB0 + st * 2 * C::B_BYTES + C::B_BYTES);
+        commit(&bar->dp_full);
+        if (!KV) commit(&bar->b2_empty[st]);
+        if (i + 1 == n) commit(&bar->a_empty[ab]);
+        return true;
+      };
+      if (!do_s(0) || !do_dp(0)) break;
+      bool ok = true;
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = (fill + i) % STAGES;
+        const uint32_t b1 = sB0 + st * 2 * C::B_BYTES, b2 = b1 + C::B_BYTES;
+        if (!wait(&bar->p_full, p_ph)) { ok = false; break; }
+        p_ph ^= 1u;
+        if (i == 0) {
+          if (!wait(&bar->acc_empty, acc_ph)) { ok = false; break; }
+          acc_ph ^= 1u;
+        }
+        tc_fence_after();
+        if constexpr (KV) {
+          issue_acc(tmem_base + C::TM_ACC1, tmem_base + C::TM_S, b2 + dh_off, i > 0);
+          commit(&bar->b2_empty[st]);
+        }
+        // S(i+1) runs while the element-wise warps turn dP(i) into dS(i).  One
+        // stage only: its tile B1 takes the place of the one dS(i) still needs.
+        if (STAGES > 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+        if (!wait(&bar->ds_full, ds_ph)) { ok = false; break; }
+        ds_ph ^= 1u;
+        tc_fence_after();
+        issue_acc(tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, b1 + dh_off, i > 0);
+        commit(&bar->b1_empty[st]);
+        if (i + 1 == n) commit(&bar->acc_full);
+        if (STAGES == 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+        if (i + 1 < n && !do_dp(i + 1)) { ok = false; break; }
+      }
+      if (!ok) break;
+      fill += n;
+    }
+  } else {
+    // ------------------------------------------------------------ element-wise warps + epilogue
+    const int g = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off + C::TM_S + g * NC;
+    const uint32_t tDP = tmem_base + lane_off + C::TM_DP + g * NC;
+    const float sl2 = p.scale_log2;
+    constexpr float kInv = BwdScale<BF16>::kInv;
+    uint32_t fill = 0, ph = 0, acc_ph = 0;
+    auto arrive = [&](uint64_t* b) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+    BwdItem it;
+    for (uint32_t ring = 0; take_item(ring, it); ++ring) {
+      const int n = it.heads * it.nt0 + it.nt1;
+      float2 rs = make_float2(0.f, 0.f);
+      if (!KV && row < it.valid) rs = __ldg(p.stats + it.out_row + row);
+      for (int i = 0; i < n; ++i, ++fill) {
+        const int stg = fill % STAGES;
+        const float* ss = sStat + stg * 2 * BN + g * NC;
+        if (KV && !wait(&bar->b1_full[stg], (fill / STAGES) & 1u)) break;
+        if (!wait(&bar->s_full, ph)) break;
+        tc_fence_after();
+        // Columns in chunks of 32, each stored as soon as it is packed: P stays
+        // in registers for dS, so the budget (168: three warps share a quarter
+        // of the register file) leaves room for one chunk of scores beside it.
+        float pr[NC];
+#pragma unroll
+        for (int h = 0; h < NC; h += 32) {
+          uint32_t x[32];
+          tmem_ld_x32(tS + h, x);
+          if constexpr (KV) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 nl = *reinterpret_cast<const float4*>(ss + h + c);
+              pr[h + c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, nl.x));
+              pr[h + c + 1] = ex2_approx(fmaf(__uint_as_float(x[c + 1]), sl2, nl.y));
+              pr[h + c + 2] = ex2_approx(fmaf(__uint_as_float(x[c + 2]), sl2, nl.z));
+              pr[h + c + 3] = ex2_approx(fmaf(__uint_as_float(x[c + 3]), sl2, nl.w));
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) pk[c] = pack2<BF16>(pr[h + 2 * c], pr[h + 2 * c + 1]);
+            tmem_st_x16_nowait(tS + h / 2, pk);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pr[h + c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, rs.x));
+          }
+        }
+        if constexpr (KV) {
+          tmem_wait_st();
+        } else {
+          const bool second = i >= it.nt0;
+          const int valid = (second ? it.end1 - (it.row1 + (i - it.nt0) * BN) : it.end0 - (it.row0 + i * BN)) - g * NC;
+          if (valid < NC) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              if (c >= valid) pr[c] = 0.f;
+          }
+        }
+        arrive(&bar->p_full);  // KV: P is written.  Q: S is read
+        if (!wait(&bar->dp_full, ph)) break;
+        tc_fence_after();
+        ph ^= 1u;
+#pragma unroll
+        for (int h = 0; h < NC; h += 32) {
+          uint32_t x[32], pk[16];
+          tmem_ld_x32(tDP + h, x);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            float4 nd;
+            if constexpr (KV) nd = *reinterpret_cast<const float4*>(ss + BN + h + c);
+            else nd = make_float4(rs.y, rs.y, rs.y, rs.y);
+            pk[c / 2] = pack2<BF16>(pr[h + c] * fmaf(__uint_as_float(x[c]), kInv, nd.x),
+                                    pr[h + c + 1] * fmaf(__uint_as_float(x[c + 1]), kInv, nd.y));
+            pk[c / 2 + 1] = pack2<BF16>(pr[h + c + 2] * fmaf(__uint_as_float(x[c + 2]), kInv, nd.z),
+                                        pr[h + c + 3] * fmaf(__uint_as_float(x[c + 3]), kInv, nd.w));
+          }
+          tmem_st_x16_nowait(tDP + h / 2, pk);
+        }
+        tmem_wait_st();
+        arrive(&bar->ds_full);
+      }
+      if (failed) break;
+      // epilogue: accumulators -> global.  KV: warps 0-3 dV, 4-7 dK; Q: the two halves of dQ's columns
+      if (n > 0) {
+        if (!wait(&bar->acc_full, acc_ph)) break;
+        acc_ph ^= 1u;
+        tc_fence_after();
+      }
+      constexpr int COLS = KV ? C::DV : (D >= 32 ? D / 2 : D);  // columns per warp
+      constexpr int OC = COLS >= 32 ? 32 : 16;
+      const bool mine = KV || D >= 32 || g == 0;
+      if (mine) {
+        const uint32_t tO = tmem_base + lane_off + (KV ? (g == 0 ? C::TM_ACC1 : C::TM_ACC2) : C::TM_ACC2 + g * COLS);
+        const float f = KV && g == 0 ? kInv : p.scale;
+        T* base = reinterpret_cast<T*>(KV ? (g == 0 ? (it.a_map ? p.dvc : p.dv) : (it.a_map ? p.dkc : p.dk)) : p.dq);
+        T* dst = base + (it.out_row + row) * (long long)D + (KV ? it.dh * C::DV : g * COLS);
+#pragma unroll 1
+        for (int c0 = 0; c0 < COLS; c0 += OC) {
+          uint32_t o[OC];
+          if (n > 0) {
+            if constexpr (OC == 32) tmem_ld_x32(tO + c0, o); else tmem_ld_x16(tO + c0, o);
+          }
+          if (row < it.limit) {
+            const bool live = n > 0 && row < it.valid;
+            uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
+#pragma unroll
+            for (int q = 0; q < OC / 8; ++q) {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = live ? pack2<BF16>(__uint_as_float(o[8 * q + 2 * e]) * f, __uint_as_float(o[8 * q + 2 * e + 1]) * f)
+                            : 0u;
+              d4[q] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      }
+      if (n > 0) arrive(&bar->acc_empty);
+    }
+  }
+
+  // ------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == C::MMA_WARP) {
+    if (*abort_flag) {
+      // Give in-flight MMAs a bounded chance to retire before freeing TMEM.
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 1000000ull) {}
+    }
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O) * 2^-kPExp}; also
+// zeroes the item counters of the two passes that follow.  Reads O and dO
+// once (bound by HBM).  delta uses the 16-bit O that the forward pass returned:
+// its rounding (half a step per element) enters dS as |dO| * 2^-9 noise, below
+// that of dS's own rounding to 16 bits.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const uint4* __restrict__ out,
+                                                             const uint4* __restrict__ dout,
+                                                             const float* __restrict__ lse, long long rows,
+                                                             float2* __restrict__ stats, int* counters) {
+  constexpr int LANES = D / 8;  // 16-byte vectors per row
+  if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long r = i / LANES;
+  float s = 0.f;
+  if (r < rows) {
+    const uint4 a = __ldg(out + i), b = __ldg(dout + i);
+    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float2 x, y;
+      if constexpr (BF16) {
+        x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&av[e]));
+        y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&bv[e]));
+      } else {
+        x = __half22float2(*reinterpret_cast<const __half2*>(&av[e]));
+        y = __half22float2(*reinterpret_cast<const __half2*>(&bv[e]));
+      }
+      s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (r < rows && threadIdx.x % LANES == 0)
+    stats[r] = make_float2(fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp), -s * BwdScale<BF16>::kInv);
+}
+
+}  // namespace fmlm

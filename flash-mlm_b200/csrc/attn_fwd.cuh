@@ -58,6 +58,10 @@ struct AttnParams {
   const int* ctx_index;  // packed, optional: context entry of each query batch
   int* work;        // packed: schedule workspace (layout at kWorkHeader)
   void* out;        // [rows, D]
+  float* lse;       // training: natural log of the softmax denominator of every output row (nullptr: not written)
+  int kv_group;     // query heads per key/value head (1 but in training)
+  int isolate;      // training: clear the V rows past a key segment's end wherever they lie (another
+                    // sequence's rows may hold NaN, and P = 0 times NaN is not 0)
   int* err;         // device error word
   const uint16_t* q_ptr;          // TQ: q itself (16-bit elements), read by the softmax warps
   long long q_sb, q_sh, q_sr;     // its batch / head / row strides in elements
@@ -301,10 +305,10 @@ __device__ __forceinline__ Item decode_item(const AttnParams& p, int w) {
       it.out_row0 = (long long)h * p.t_out + seq_start + rel0;
     }
   }
-  const int kh = p.is_mla ? 0 : h;
+  const int kh = p.is_mla ? 0 : h / p.kv_group;
   // context segment
   Seg& c = it.ctx;
-  c.map = 0; c.h = kh; c.fix = 0;
+  c.map = 0; c.h = kh; c.fix = p.isolate;
   if (!p.has_ctx) {
     c.b = 0; c.row0 = 0; c.row1 = 0;
   } else if (p.mode == 0) {
@@ -322,12 +326,12 @@ __device__ __forceinline__ Item decode_item(const AttnParams& p, int w) {
   Seg& m = it.main;
   m.map = 1; m.fix = 0;
   if (p.mode == 0) {
-    m.h = h;  // dense MLA attends the per-head keys (mlm_kernel_impl.py:124, :188-206)
+    m.h = p.is_mla ? h : kh;  // dense MLA attends the per-head keys (mlm_kernel_impl.py:124, :188-206)
     m.b = b; m.row0 = 0; m.row1 = p.N;
   } else if (p.main_padded) {
     m.h = kh; m.b = b; m.row0 = 0; m.row1 = L; m.fix = (L < p.N);
   } else {
-    m.h = kh; m.b = 0; m.row0 = p.causal ? 0 : seq_start; m.row1 = seq_start + L;
+    m.h = kh; m.b = 0; m.row0 = p.causal ? 0 : seq_start; m.row1 = seq_start + L; m.fix = p.isolate;
   }
   c.nblk = c.row1 > c.row0 ? (c.row1 - c.row0 + BN - 1) / BN : 0;
   m.nblk = m.row1 > m.row0 ? (m.row1 - m.row0 + BN - 1) / BN : 0;
@@ -1314,6 +1318,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NQ>::THREADS) __maxnreg__((AttnCfg<
       tc_fence_after();
       const float inv = (l > 0.f) ? 1.0f / l : 1.0f;
       T* orow = out + (it.out_row0 + t * BM + row) * (long long)D + it.dh() * C::DV;
+      // m is in units of log2: lse = ln 2 * (m + log2 l)
+      if (p.lse != nullptr && row_valid)
+        p.lse[it.out_row0 + t * BM + row] = l > 0.f ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
       auto store_chunk = [&](const uint32_t(&o)[OC], int c0) {
         if (!row_valid) return;
         uint32_t v[OC / 2];

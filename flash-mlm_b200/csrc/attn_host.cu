@@ -1,13 +1,12 @@
 // C-ABI entry points for the attention forward path: argument validation,
 // TMA tensor-map encoding, the on-device tile scheduler and kernel dispatch.
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <cmath>
 #include <mutex>
 
 #include "attn_fwd.cuh"
 #include "common.h"
+#include "tma_map.h"
 
 namespace fmlm {
 
@@ -30,62 +29,6 @@ int device_sm_count() {
 }
 
 namespace {
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
-}
-
-// Encodes a 4-D tiled map {D, rows, heads, batch} over `v` with a box of
-// {swizzle_bytes / 2, box_rows, 1, 1} and the matching shared-memory swizzle.
-// Empty views get a 1-row map over `fallback` that the kernel never loads.
-int encode_view(CUtensorMap* m, const fmlm_view4& v, int D, int box_rows, int dtype, const void* fallback,
-                const char* name) {
-  auto enc = encode_fn();
-  if (!enc) return set_error(FMLM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  const int swb = std::min(128, D * 2);
-  const bool empty = v.data == nullptr || v.rows <= 0 || v.heads <= 0 || v.batch <= 0;
-  const void* base = empty ? fallback : v.data;
-  if (!aligned16(base)) return set_error(FMLM_ERR_INVALID, "%s: base address must be 16-byte aligned", name);
-  cuuint64_t dims[4], strides[3];
-  dims[0] = static_cast<cuuint64_t>(D);
-  dims[1] = empty ? 1 : static_cast<cuuint64_t>(v.rows);
-  dims[2] = empty ? 1 : static_cast<cuuint64_t>(v.heads);
-  dims[3] = empty ? 1 : static_cast<cuuint64_t>(v.batch);
-  const int64_t rs = empty ? D : v.row_stride;
-  int64_t hs = empty ? D : v.head_stride;
-  int64_t bs = empty ? D : v.batch_stride;
-  if (!empty) {
-    if (rs < D || (rs * 2) % 16 != 0) return set_error(FMLM_ERR_INVALID, "%s: row stride must be >= head_dim and a multiple of 8 elements", name);
-    if (v.heads == 1 && (hs <= 0 || (hs * 2) % 16 != 0)) hs = rs * v.rows;
-    if (v.batch == 1 && (bs <= 0 || (bs * 2) % 16 != 0)) bs = hs * v.heads;
-    if ((hs * 2) % 16 != 0 || hs <= 0 || (bs * 2) % 16 != 0 || bs <= 0)
-      return set_error(FMLM_ERR_INVALID, "%s: head/batch strides must be positive multiples of 8 elements", name);
-  }
-  strides[0] = static_cast<cuuint64_t>(rs) * 2;
-  strides[1] = static_cast<cuuint64_t>(hs) * 2;
-  strides[2] = static_cast<cuuint64_t>(bs) * 2;
-  cuuint32_t box[4] = {static_cast<cuuint32_t>(swb / 2), static_cast<cuuint32_t>(box_rows), 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle sw = swb == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                : swb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                            : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUtensorMapDataType dt =
-      dtype == FMLM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  CUresult r = enc(m, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(FMLM_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", name, (int)r);
-  return FMLM_OK;
-}
 
 // Builds the packed-mode work list: one entry per (sequence, query pair of
 // PAIR rows), sequences ordered by decreasing key count (longest first) so
@@ -270,12 +213,26 @@ int check_common(int dtype, int D, const void* out) {
   return FMLM_OK;
 }
 
-}  // namespace
-}  // namespace fmlm
+// What the training forms of the launchers add to the inference forms.
+struct TrainExtras {
+  int kv_heads = 0;      // heads of k / v (0: as many as q has)
+  float* lse = nullptr;  // natural log of each row's softmax denominator, in output-row order
+};
 
-using namespace fmlm;
+// Fills the training fields of `p`; checks the head counts.
+int apply_extras(AttnParams& p, const TrainExtras& x) {
+  p.kv_group = 1;
+  if (x.kv_heads > 0) {
+    if (p.is_mla || p.H % x.kv_heads != 0)
+      return set_error(FMLM_ERR_INVALID, "num_heads (%d) must be a multiple of kv_heads (%d), without MLA", p.H, x.kv_heads);
+    p.kv_group = p.H / x.kv_heads;
+  }
+  p.lse = x.lse;
+  p.isolate = x.lse != nullptr;
+  return FMLM_OK;
+}
 
-extern "C" int fmlm_attn_dense_fwd(const fmlm_dense_args* a, void* stream) {
+int dense_fwd(const fmlm_dense_args* a, const TrainExtras& x, void* stream) {
   if (!a) return set_error(FMLM_ERR_INVALID, "null args");
   int rc = check_common(a->dtype, a->head_dim, a->out);
   if (rc) return rc;
@@ -316,6 +273,7 @@ extern "C" int fmlm_attn_dense_fwd(const fmlm_dense_args* a, void* stream) {
   p.q_sh = a->q.head_stride;
   p.q_sr = a->q.row_stride;
   p.timeout_ns = kTimeoutNs;
+  if ((rc = apply_extras(p, x))) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->dtype == FMLM_DTYPE_BF16 ? dispatch<true>(D, m, p, items, s) : dispatch<false>(D, m, p, items, s);
 }
@@ -330,6 +288,11 @@ bool packed_single_tile(int D, int64_t total_q_len, int batch, int heads) {
          (total_q_len / pair_rows(D) + batch) * (int64_t)heads < (int64_t)FMLM_SINGLE_TILE_FACTOR * device_sm_count();
 }
 
+}  // namespace
+}  // namespace fmlm
+
+using namespace fmlm;
+
 extern "C" size_t fmlm_packed_workspace_bytes(int32_t batch, int64_t total_q_len, int32_t head_dim) {
   // sized for the finer of the two item granularities head_dim 128 may use
   const int64_t pr = head_dim > 0 ? (head_dim == 128 ? 128 : pair_rows(head_dim)) : 128;
@@ -337,7 +300,10 @@ extern "C" size_t fmlm_packed_workspace_bytes(int32_t batch, int64_t total_q_len
   return (size_t)((cap + kWorkHeader) * sizeof(int32_t) + 15) / 16 * 16;
 }
 
-extern "C" int fmlm_attn_packed_fwd(const fmlm_packed_args* a, void* stream) {
+namespace fmlm {
+namespace {
+
+int packed_fwd(const fmlm_packed_args* a, const TrainExtras& x, void* stream) {
   if (!a) return set_error(FMLM_ERR_INVALID, "null args");
   int rc = check_common(a->dtype, a->head_dim, a->out);
   if (rc) return rc;
@@ -419,9 +385,35 @@ extern "C" int fmlm_attn_packed_fwd(const fmlm_packed_args* a, void* stream) {
 #ifdef FMLM_TRACE
   p.trace = g_trace_buffer;
 #endif
+  if ((rc = apply_extras(p, x))) return rc;
   const long long items_bound = cap * (long long)a->num_heads * o_halves(D);
   return a->dtype == FMLM_DTYPE_BF16 ? dispatch<true>(D, m, p, items_bound, s, single)
                                      : dispatch<false>(D, m, p, items_bound, s, single);
+}
+
+}  // namespace
+}  // namespace fmlm
+
+extern "C" int fmlm_attn_dense_fwd(const fmlm_dense_args* a, void* stream) { return dense_fwd(a, TrainExtras(), stream); }
+
+extern "C" int fmlm_attn_packed_fwd(const fmlm_packed_args* a, void* stream) {
+  return packed_fwd(a, TrainExtras(), stream);
+}
+
+extern "C" int fmlm_attn_dense_fwd_lse(const fmlm_dense_args* a, int32_t kv_heads, float* lse, void* stream) {
+  if (!a || !lse || kv_heads < 1) return set_error(FMLM_ERR_INVALID, "args, lse and kv_heads >= 1 are required");
+  TrainExtras x;
+  x.kv_heads = kv_heads;
+  x.lse = lse;
+  return dense_fwd(a, x, stream);
+}
+
+extern "C" int fmlm_attn_packed_fwd_lse(const fmlm_packed_args* a, int32_t kv_heads, float* lse, void* stream) {
+  if (!a || !lse || kv_heads < 1) return set_error(FMLM_ERR_INVALID, "args, lse and kv_heads >= 1 are required");
+  TrainExtras x;
+  x.kv_heads = kv_heads;
+  x.lse = lse;
+  return packed_fwd(a, x, stream);
 }
 
 #ifdef FMLM_TRACE

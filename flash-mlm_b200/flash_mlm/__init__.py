@@ -9,6 +9,7 @@ or without the built library raises instead of falling back.
 from flash_mlm.host.cache import InferenceCache, PackMetadata, PackingCache
 from flash_mlm.host.host import flash_attn_mlm, flash_attn_mlm_compressed, flash_attn_mlm_precompressed
 from flash_mlm.host.host_utils import build_pack_metadata, unpack_from_kernel
+from flash_mlm.host.train import flash_attn_mlm_bwd, flash_attn_mlm_fwd, flash_attn_mlm_train
 from flash_mlm._lib import check_device_errors
 
 __all__ = [
@@ -20,4 +21,7 @@ __all__ = [
     "flash_attn_mlm",
     "flash_attn_mlm_compressed",
     "flash_attn_mlm_precompressed",
+    "flash_attn_mlm_train",
+    "flash_attn_mlm_fwd",
+    "flash_attn_mlm_bwd",
 ]

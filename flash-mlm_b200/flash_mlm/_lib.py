@@ -89,6 +89,46 @@ class PackedArgs(ctypes.Structure):
     ]
 
 
+FMLM_BWD_DENSE = 0
+FMLM_BWD_PADDED = 1
+FMLM_BWD_PACKED = 2
+
+
+class AttnBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("causal_query_seq_attn", ctypes.c_int32),
+        ("context_entries", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("total_q_len", ctypes.c_int64),
+        ("total_context_len", ctypes.c_int64),
+        ("q", View4),
+        ("k", View4),
+        ("v", View4),
+        ("dout", View4),
+        ("k_context", View4),
+        ("v_context", View4),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("cu_seqlens_q", ctypes.c_void_p),
+        ("cu_seqlens_context", ctypes.c_void_p),
+        ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p),
+        ("dv", ctypes.c_void_p),
+        ("dk_context", ctypes.c_void_p),
+        ("dv_context", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("error_word", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -115,6 +155,14 @@ def lib() -> ctypes.CDLL:
         L.fmlm_attn_packed_fwd.restype = ctypes.c_int
         L.fmlm_attn_packed_fwd_noalloc.argtypes = [ctypes.POINTER(PackedArgs), vp]
         L.fmlm_attn_packed_fwd_noalloc.restype = ctypes.c_int
+        L.fmlm_attn_dense_fwd_lse.argtypes = [ctypes.POINTER(DenseArgs), i32, vp, vp]
+        L.fmlm_attn_dense_fwd_lse.restype = ctypes.c_int
+        L.fmlm_attn_packed_fwd_lse.argtypes = [ctypes.POINTER(PackedArgs), i32, vp, vp]
+        L.fmlm_attn_packed_fwd_lse.restype = ctypes.c_int
+        L.fmlm_attn_bwd.argtypes = [ctypes.POINTER(AttnBwdArgs), vp]
+        L.fmlm_attn_bwd.restype = ctypes.c_int
+        L.fmlm_attn_bwd_workspace_bytes.argtypes = [i64]
+        L.fmlm_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.fmlm_selftest_bounded_wait.argtypes = [vp, ctypes.c_uint64, vp]
         L.fmlm_selftest_bounded_wait.restype = ctypes.c_int
         L.fmlm_packed_workspace_bytes.argtypes = [i32, i64, i32]

@@ -1,0 +1,333 @@
+"""Attention for training: the forward pass with its softmax statistics, the
+backward pass, and a differentiable call over both.
+
+No counterpart in the reference, whose kernels are forward only (its README
+lists the backward pass as planned).  The attention pattern is that of
+``flash_attn_mlm`` and ``flash_attn_mlm_compressed``: every query attends to
+its context (one shared by the batch, or one per sequence), then to its own
+sequence, or with ``causal_query_seq_attn`` to all sequences up to its own.
+Here the context keys and values are arguments, since a training step
+computes them and wants their gradients.
+
+Three layouts:
+
+* dense: q [B, H, N, D], no ``q_meta``: every token is valid;
+* padded: q [B, H, N, D] with ``q_meta``: the first ``lengths[b]`` tokens are valid;
+* packed: q [H, T, D] with ``q_meta`` of T tokens (what ``pack_for_kernel`` returns).
+
+k and v may have fewer heads than q (a divisor): query head h attends key head
+``h // (H // HK)`` and the gradients of a shared head are summed.  Inputs may
+have any strides whose last one is 1; others, and tensors that the TMA unit
+cannot address, are copied.  Gradients are deterministic: the same inputs give
+the same bits.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from flash_mlm import _lib
+from flash_mlm.host.cache import PackMetadata
+from flash_mlm.host.host_utils import pack_for_kernel, require_cuda_tensors, unpack_from_kernel, validate_head_dim_supported
+
+
+def _tma_ready(x: torch.Tensor) -> torch.Tensor:
+    """x itself if TMA can address its rows (16-byte aligned, positive strides), else a contiguous copy."""
+    d = x.shape[-1]
+    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and x.stride(-2) >= d and x.stride(-2) % 8 == 0
+    for size, stride in zip(x.shape[:-2], x.stride()[:-2]):
+        ok = ok and (size == 1 or (stride > 0 and stride % 8 == 0))
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def _view(x: torch.Tensor) -> _lib.View4:
+    """[B, H, N, D] or [H, T, D] as a [batch][heads][rows] view."""
+    if x.ndim == 4:
+        return _lib.view_bhnd(x)
+    h, t, d = x.shape
+    return _lib.view4(x, rows=t, heads=h, batch=1, row_stride=x.stride(1), head_stride=x.stride(0),
+                      batch_stride=h * t * d)
+
+
+def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
+    """Shapes, types and devices of a training call; returns the layout code."""
+    if q.ndim not in (3, 4) or k.ndim != q.ndim or v.ndim != q.ndim:
+        raise ValueError("q/k/v must be rank-4 tensors [B, H, N, D] or packed rank-3 tensors [H, T, D]")
+    if k.shape != v.shape:
+        raise ValueError("k and v must have the same shape")
+    hdim = q.ndim - 3
+    if q.shape[:hdim] != k.shape[:hdim] or q.shape[hdim + 1:] != k.shape[hdim + 1:]:
+        raise ValueError("q and k may differ in their number of heads only")
+    h, hk = q.shape[hdim], k.shape[hdim]
+    if hk < 1 or h < 1 or h % hk != 0:
+        raise ValueError("the heads of q must be a multiple of the heads of k and v")
+    validate_head_dim_supported(q.shape[-1])
+    _lib.dtype_code(q.dtype)
+    packed = q.ndim == 3
+    if packed:
+        if q_meta is None:
+            raise ValueError("packed q/k/v need q_meta")
+        if q_meta.total_tokens != q.shape[1]:
+            raise ValueError("packed token count mismatch with PackMetadata")
+    elif q_meta is not None and (q_meta.B != q.shape[0] or q_meta.N != q.shape[2]):
+        raise ValueError("q_meta shape metadata does not match q/k/v padded shape")
+    given = [x is not None for x in (context_k, context_v, context_meta)]
+    if any(given) and not all(given):
+        raise ValueError("context_k, context_v and context_meta must be provided together or all omitted")
+    if (all(given) or causal) and q_meta is None:
+        raise ValueError("a context and causal_query_seq_attn need q_meta")
+    tensors = [q, k, v]
+    if all(given):
+        d = q.shape[-1]
+        if context_k.shape != (hk, context_meta.total_tokens, d) or context_v.shape != context_k.shape:
+            raise ValueError("context_k and context_v must be [heads of k, context_meta.total_tokens, D]")
+        if context_meta.B not in (1, q_meta.B):
+            raise ValueError("context_meta must describe one context, or one for every sequence")
+        tensors += [context_k, context_v]
+    if any(x.dtype != q.dtype for x in tensors):
+        raise ValueError("q, k, v and the context must have the same dtype")
+    if any(x.device != q.device for x in tensors):
+        raise ValueError("q, k, v and the context must be on the same device")
+    metas = [m.cu_seqlens for m in (q_meta, context_meta) if m is not None]
+    require_cuda_tensors(*tensors, *metas)
+    if any(m.device != q.device for m in metas):
+        raise ValueError("q_meta and context_meta must be on q's device")
+    if any(m.dtype != torch.int32 or not m.is_contiguous() for m in metas):
+        raise ValueError("cu_seqlens must be contiguous int32")
+    if packed:
+        return _lib.FMLM_BWD_PACKED
+    return _lib.FMLM_BWD_DENSE if q_meta is None else _lib.FMLM_BWD_PADDED
+
+
+def _require_packed(q, context_k, causal):
+    if q.ndim != 3 and (context_k is not None or causal):
+        raise ValueError("a context and causal_query_seq_attn need packed q/k/v [H, T, D] here "
+                         "(pack_for_kernel packs; flash_attn_mlm_train does it itself)")
+
+
+def _nothing_to_do(q: torch.Tensor, q_meta: PackMetadata | None) -> bool:
+    return q.numel() == 0 or (q_meta is not None and q_meta.total_tokens == 0)
+
+
+def flash_attn_mlm_fwd(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float,
+    q_meta: PackMetadata | None = None,
+    context_k: torch.Tensor | None = None,
+    context_v: torch.Tensor | None = None,
+    context_meta: PackMetadata | None = None,
+    causal_query_seq_attn: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention output and softmax statistics for ``flash_attn_mlm_bwd``.
+
+    q [B, H, N, D] (dense, or padded with ``q_meta``) or [H, T, D] (packed);
+    k, v: the same with a divisor of H as heads.  ``context_k`` / ``context_v``
+    [HK, Tc, D] with ``context_meta`` (of one context, or of one per sequence)
+    and ``causal_query_seq_attn`` need the packed layout.
+
+    Returns out (q's shape and dtype, contiguous; zero rows past each sequence)
+    and lse (float32, q's shape without D): the natural log of each row's
+    softmax denominator, undefined at padding rows.
+    """
+    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    _require_packed(q, context_k, causal_query_seq_attn)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+    if _nothing_to_do(q, q_meta):
+        return out.zero_(), lse.fill_(float("-inf"))
+    q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
+    h, d, hk = q.shape[-3], q.shape[-1], k.shape[-3]
+    L = _lib.lib()
+    err = _lib.error_word(q.device)
+    if layout == _lib.FMLM_BWD_DENSE:
+        args = _lib.DenseArgs()
+        args.dtype, args.head_dim = _lib.dtype_code(q.dtype), d
+        args.batch, args.num_heads, args.seq_len = q.shape[0], h, q.shape[2]
+        args.context_batch_size = 1
+        args.scale = float(scale)
+        args.q, args.k, args.v = _view(q), _view(k), _view(v)
+        args.out, args.error_word = out.data_ptr(), err.data_ptr()
+        launch = L.fmlm_attn_dense_fwd_lse
+    else:
+        packed = layout == _lib.FMLM_BWD_PACKED
+        args = _lib.PackedArgs()
+        args.dtype, args.head_dim, args.num_heads, args.batch = _lib.dtype_code(q.dtype), d, h, q_meta.B
+        args.causal_query_seq_attn = int(causal_query_seq_attn)
+        args.context_batch_size = 1
+        args.scale = float(scale)
+        args.q_layout = args.kv_layout = _lib.FMLM_LAYOUT_PACKED if packed else _lib.FMLM_LAYOUT_PADDED
+        args.seq_len = 0 if packed else q.shape[2]
+        args.total_q_len = q_meta.total_tokens
+        args.q, args.k, args.v = _view(q), _view(k), _view(v)
+        args.cu_seqlens_q = q_meta.cu_seqlens.data_ptr()
+        if context_k is not None and context_meta.total_tokens > 0:
+            context_k, context_v = _tma_ready(context_k), _tma_ready(context_v)
+            args.k_cache, args.v_cache = _view(context_k), _view(context_v)
+            args.cu_seqlens_kv = context_meta.cu_seqlens.data_ptr()
+            args.context_batch_size = context_meta.B
+        args.out, args.out_rows_per_head, args.out_padded = out.data_ptr(), q_meta.total_tokens, int(not packed)
+        nbytes = L.fmlm_packed_workspace_bytes(q_meta.B, q_meta.total_tokens, d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        args.workspace, args.workspace_bytes, args.error_word = ws.data_ptr(), nbytes, err.data_ptr()
+        launch = L.fmlm_attn_packed_fwd_lse
+    with torch.cuda.device(q.device):
+        _lib.check(launch(ctypes.byref(args), hk, lse.data_ptr(), _lib.stream_ptr(q.device)), "flash_attn_mlm_fwd")
+    return out, lse
+
+
+def flash_attn_mlm_bwd(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    scale: float,
+    q_meta: PackMetadata | None = None,
+    context_k: torch.Tensor | None = None,
+    context_v: torch.Tensor | None = None,
+    context_meta: PackMetadata | None = None,
+    causal_query_seq_attn: bool = False,
+    need_dq: bool = True,
+    need_dkv: bool = True,
+) -> tuple[torch.Tensor | None, ...]:
+    """Gradients (dq, dk, dv, dcontext_k, dcontext_v) of ``flash_attn_mlm_fwd``.
+
+    ``out`` and ``lse`` are what the forward call returned for the same
+    arguments, ``dout`` the gradient of ``out``.  Gradients have their
+    tensors' shapes and dtypes, contiguous, with zero rows past each sequence.
+    What is not needed (``need_dq``, ``need_dkv``), and the context's without
+    a context, is None.
+    """
+    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    _require_packed(q, context_k, causal_query_seq_attn)
+    for name, x in (("dout", dout), ("out", out)):
+        if x.shape != q.shape or x.dtype != q.dtype or x.device != q.device:
+            raise ValueError(f"{name} must have q's shape, dtype and device")
+    if lse.shape != q.shape[:-1] or lse.dtype != torch.float32 or lse.device != q.device:
+        raise ValueError("lse must be float32 of q's shape without the head dimension, on q's device")
+    dev = q.device
+
+    def like(x, wanted):
+        return torch.empty(x.shape, dtype=x.dtype, device=dev) if wanted and x is not None else None
+
+    dq, dk, dv = like(q, need_dq), like(k, need_dkv), like(v, need_dkv)
+    dkc, dvc = like(context_k, need_dkv), like(context_v, need_dkv)
+    grads = (dq, dk, dv, dkc, dvc)
+    if not (need_dq or need_dkv):
+        return grads
+    if _nothing_to_do(q, q_meta):
+        for g in grads:
+            if g is not None:
+                g.zero_()
+        return grads
+    q, k, v, dout = (_tma_ready(x) for x in (q, k, v, dout))
+    dout, out, lse = _tma_ready(dout.contiguous()), _tma_ready(out.contiguous()), lse.contiguous()
+    packed = layout == _lib.FMLM_BWD_PACKED
+    L = _lib.lib()
+    args = _lib.AttnBwdArgs()
+    args.dtype, args.head_dim, args.layout = _lib.dtype_code(q.dtype), q.shape[-1], layout
+    args.batch = q_meta.B if packed else q.shape[0]
+    args.num_heads, args.kv_heads = q.shape[-3], k.shape[-3]
+    args.seq_len = 0 if packed else q.shape[2]
+    args.causal_query_seq_attn = int(causal_query_seq_attn)
+    args.scale = float(scale)
+    args.total_q_len = q.shape[1] if packed else 0
+    args.q, args.k, args.v, args.dout = _view(q), _view(k), _view(v), _view(dout)
+    if q_meta is not None:
+        args.cu_seqlens_q = q_meta.cu_seqlens.data_ptr()
+    if context_k is not None and context_meta.total_tokens > 0:
+        context_k, context_v = _tma_ready(context_k), _tma_ready(context_v)
+        args.context_entries, args.total_context_len = context_meta.B, context_meta.total_tokens
+        args.k_context, args.v_context = _view(context_k), _view(context_v)
+        args.cu_seqlens_context = context_meta.cu_seqlens.data_ptr()
+    args.out, args.lse = out.data_ptr(), lse.data_ptr()
+    args.dq, args.dk, args.dv, args.dk_context, args.dv_context = (None if g is None else g.data_ptr() for g in grads)
+    nbytes = L.fmlm_attn_bwd_workspace_bytes(lse.numel())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    args.error_word = _lib.error_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        _lib.check(L.fmlm_attn_bwd(ctypes.byref(args), _lib.stream_ptr(dev)), "flash_attn_mlm_bwd")
+    return grads
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, context_k, context_v, scale, q_meta, context_meta, causal):
+        out, lse = flash_attn_mlm_fwd(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal)
+        ctx.save_for_backward(q, k, v, context_k, context_v, out, lse)
+        ctx.call = (scale, q_meta, context_meta, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, context_k, context_v, out, lse = ctx.saved_tensors
+        scale, q_meta, context_meta, causal = ctx.call
+        need = ctx.needs_input_grad
+        grads = flash_attn_mlm_bwd(dout, q, k, v, out, lse, scale, q_meta, context_k, context_v, context_meta, causal,
+                                   need_dq=need[0], need_dkv=any(need[1:5]))
+        return (*grads, None, None, None, None)
+
+
+class _Pack(torch.autograd.Function):
+    """Padded [B, H, N, D] -> packed [H, T, D]; the gradient is unpacked."""
+
+    @staticmethod
+    def forward(ctx, x, meta):
+        ctx.meta = meta
+        return pack_for_kernel(x, meta)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return unpack_from_kernel(g, ctx.meta, g.shape[0]), None
+
+
+class _Unpack(torch.autograd.Function):
+    """Packed [H, T, D] -> padded [B, H, N, D]; the gradient is packed."""
+
+    @staticmethod
+    def forward(ctx, x, meta):
+        ctx.meta = meta
+        return unpack_from_kernel(x, meta, x.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return pack_for_kernel(g, ctx.meta), None
+
+
+def flash_attn_mlm_train(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float,
+    q_meta: PackMetadata | None = None,
+    context_k: torch.Tensor | None = None,
+    context_v: torch.Tensor | None = None,
+    context_meta: PackMetadata | None = None,
+    causal_query_seq_attn: bool = False,
+) -> torch.Tensor:
+    """Differentiable attention (``flash_attn_mlm_fwd``, with ``flash_attn_mlm_bwd`` as its gradient).
+
+    The arguments of ``flash_attn_mlm_fwd``; padded q/k/v with a context or
+    ``causal_query_seq_attn`` are packed first (and their gradients unpacked).
+    Returns out in q's layout.  Gradients flow to q, k, v, context_k and
+    context_v.  float16: as with any float16 gradient, the products of dout
+    with v must stay inside float16's range (loss scaling sees to that).
+
+    To capture the backward pass into a CUDA graph, call ``flash_attn_mlm_fwd``
+    and ``flash_attn_mlm_bwd``, which involve no autograd graph.
+    """
+    _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    if q.ndim == 4 and (context_k is not None or causal_query_seq_attn):
+        qp, kp, vp = (_Pack.apply(x, q_meta) for x in (q, k, v))
+        out = _Attention.apply(qp, kp, vp, context_k, context_v, scale, q_meta, context_meta, causal_query_seq_attn)
+        return _Unpack.apply(out, q_meta)
+    return _Attention.apply(q, k, v, context_k, context_v, scale, q_meta, context_meta, causal_query_seq_attn)

@@ -150,6 +150,52 @@ FMLM_API int fmlm_build_pack_metadata(const int32_t* lengths, int32_t B, int32_t
                              int32_t* cu_seqlens, int64_t* token_indices, int32_t* batch_ids_q,
                              int32_t* q_tile_starts_q, int32_t* counters, void* stream);
 
+/* Training forms of the two launchers: the same computation, plus
+ *   kv_heads  heads of k / v (and of the context); num_heads must be a
+ *             multiple of it, and query head h attends head h / (num_heads / kv_heads);
+ *   lse       [output rows] float: the natural log of each row's softmax
+ *             denominator, in the order of the output's rows, for the backward pass.
+ * Rows of other sequences and of padding, NaN and infinities among them, leave
+ * a sequence's results untouched.  No MLA.  No counterpart in the reference. */
+FMLM_API int fmlm_attn_dense_fwd_lse(const fmlm_dense_args* args, int32_t kv_heads, float* lse, void* stream);
+FMLM_API int fmlm_attn_packed_fwd_lse(const fmlm_packed_args* args, int32_t kv_heads, float* lse, void* stream);
+
+enum { FMLM_BWD_DENSE = 0, FMLM_BWD_PADDED = 1, FMLM_BWD_PACKED = 2 };
+
+/* Arguments of the attention backward pass (no counterpart in the reference,
+ * whose kernels are forward only). */
+typedef struct fmlm_attn_bwd_args {
+  int32_t dtype, head_dim;          /* FMLM_DTYPE_*; 16, 32, 64, 128, 256 */
+  int32_t layout;                   /* FMLM_BWD_DENSE: [B,H,N,D], every row valid; _PADDED: [B,H,N,D] with
+                                       cu_seqlens_q; _PACKED: [H][T][D] with cu_seqlens_q (views of batch 1) */
+  int32_t batch, num_heads, kv_heads;
+  int32_t seq_len;                  /* N (dense, padded) */
+  int32_t causal_query_seq_attn;    /* packed only */
+  int32_t context_entries;          /* 0: no context; 1: one shared by all sequences; batch: one each (packed only) */
+  float scale;
+  int64_t total_q_len;              /* packed: T */
+  int64_t total_context_len;        /* rows per head of the context */
+  fmlm_view4 q, k, v, dout;         /* q, dout: num_heads heads; k, v: kv_heads */
+  fmlm_view4 k_context, v_context;  /* [kv_heads][total_context_len] */
+  const void* out;                  /* the forward's output, contiguous [B,H,N,D] or [H,T,D] */
+  const float* lse;                 /* the forward's lse, in the order of out's rows */
+  const int32_t* cu_seqlens_q;      /* [batch + 1] (padded, packed) */
+  const int32_t* cu_seqlens_context;/* [context_entries + 1] */
+  void *dq, *dk, *dv;               /* contiguous, shaped like q, k, v; padding rows get zeros.  dq may be NULL, and
+                                       dk with dv (and the context's): gradients that nobody asks for */
+  void *dk_context, *dv_context;    /* contiguous [kv_heads][total_context_len][D]; rows of no entry are left unwritten */
+  void* workspace;                  /* fmlm_attn_bwd_workspace_bytes() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int32_t* error_word;
+} fmlm_attn_bwd_args;
+
+/* Gradients of q, k, v (and of the context's k, v): dq, dk, dv from dout.
+ * The same inputs give the same bits (no floating-point atomics). */
+FMLM_API int fmlm_attn_bwd(const fmlm_attn_bwd_args* args, void* stream);
+
+/* Workspace for fmlm_attn_bwd; rows = output rows (B*H*N dense or padded, H*T packed). */
+FMLM_API size_t fmlm_attn_bwd_workspace_bytes(int64_t rows);
+
 /* Gather the valid rows of x [B][H][N][D] into out [H * total_padded, D], zeroing
  * rows [total_tokens, total_padded) of every head.
  * Replaces _pack_flatten_for_kernel_into / pack_for_kernel
