@@ -9,6 +9,7 @@ or without the built library raises instead of falling back.
 from flash_mlm.host.cache import InferenceCache, PackMetadata, PackingCache
 from flash_mlm.host.host import flash_attn_mlm, flash_attn_mlm_compressed, flash_attn_mlm_precompressed
 from flash_mlm.host.host_utils import build_pack_metadata, unpack_from_kernel
+from flash_mlm.host.rope import RotaryTable, qk_norm_rope
 from flash_mlm.host.train import flash_attn_mlm_bwd, flash_attn_mlm_fwd, flash_attn_mlm_train
 from flash_mlm._lib import check_device_errors
 
@@ -24,4 +25,6 @@ __all__ = [
     "flash_attn_mlm_train",
     "flash_attn_mlm_fwd",
     "flash_attn_mlm_bwd",
+    "RotaryTable",
+    "qk_norm_rope",
 ]

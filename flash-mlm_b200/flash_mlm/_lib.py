@@ -129,6 +129,46 @@ class AttnBwdArgs(ctypes.Structure):
     ]
 
 
+FMLM_PAIRS_HALF = 0
+FMLM_PAIRS_INTERLEAVED = 1
+
+
+class QkRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("packed", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("normalize", ctypes.c_int32),
+        ("weight_f32", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("max_positions", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q", View4),
+        ("k", View4),
+        ("gq", View4),
+        ("gk", View4),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("position_offsets", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("token_indices", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("dq_weight", ctypes.c_void_p),
+        ("dk_weight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("error_word", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -163,6 +203,12 @@ def lib() -> ctypes.CDLL:
         L.fmlm_attn_bwd.restype = ctypes.c_int
         L.fmlm_attn_bwd_workspace_bytes.argtypes = [i64]
         L.fmlm_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
+        L.fmlm_qk_rope_fwd.argtypes = [ctypes.POINTER(QkRopeArgs), vp]
+        L.fmlm_qk_rope_fwd.restype = ctypes.c_int
+        L.fmlm_qk_rope_bwd.argtypes = [ctypes.POINTER(QkRopeArgs), vp]
+        L.fmlm_qk_rope_bwd.restype = ctypes.c_int
+        L.fmlm_qk_rope_bwd_workspace_bytes.argtypes = [i32]
+        L.fmlm_qk_rope_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.fmlm_selftest_bounded_wait.argtypes = [vp, ctypes.c_uint64, vp]
         L.fmlm_selftest_bounded_wait.restype = ctypes.c_int
         L.fmlm_packed_workspace_bytes.argtypes = [i32, i64, i32]
@@ -252,7 +298,8 @@ def check_device_errors(device: torch.device | None = None) -> None:
     3 = a context_index entry was out of range (that sequence attended no
     context); 4 = a packed sequence had more than 65536 work items (it was
     not computed); 5 = a cache append would have passed the cache capacity
-    (nothing was written).
+    (nothing was written); 6 = a position lay outside the rotary table (the
+    table's nearest row was used).
     """
     devs = [device] if device is not None else [torch.device("cuda", i) for i in list(_err_words)]
     for d in devs:
@@ -263,7 +310,8 @@ def check_device_errors(device: torch.device | None = None) -> None:
             what = {1: "gave up waiting", 2: "found its shared memory misaligned",
                     3: "met a context_index entry out of range",
                     4: "met a sequence too long for the tile schedule",
-                    5: "would have overrun a context cache's capacity (nothing appended)"}.get(v, "failed")
+                    5: "would have overrun a context cache's capacity (nothing appended)",
+                    6: "met a position outside the rotary table"}.get(v, "failed")
             raise FlashMLMError(f"flash_mlm kernel on {d} {what} (code {v}); results are invalid")
 
 

@@ -1,0 +1,239 @@
+"""Per-head norm of queries and keys with the position rotation in the same
+pass, in front of the attention (no counterpart in the reference).
+
+``RotaryTable`` holds the cosines and sines of every position, computed in
+float64 once (an angle of position 100000 has lost its low digits in float32);
+``qk_norm_rope`` reads q and k once and writes them once, and is differentiable
+in q, k and the norm's weights.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from flash_mlm import _lib
+from flash_mlm.host.cache import PackMetadata
+from flash_mlm.host.host_utils import require_cuda_tensors, validate_head_dim_supported
+
+_PAIRS = {"half": _lib.FMLM_PAIRS_HALF, "interleaved": _lib.FMLM_PAIRS_INTERLEAVED}
+
+
+class RotaryTable:
+    """Cosines and sines [max_positions, rotary_dim / 2, 2] (float32) of the rotation angles
+    ``position * base ** (-2 j / rotary_dim)``, or ``position * inv_freq[j]``.
+
+    ``pairs``: which columns turn together: "half" (j, j + rotary_dim / 2) or
+    "interleaved" (2 j, 2 j + 1).  ``rotary_dim`` is a multiple of 16; a head's
+    columns past it are not rotated.
+    """
+
+    def __init__(self, max_positions: int, rotary_dim: int, *, base: float = 10000.0,
+                 inv_freq: torch.Tensor | None = None, pairs: str = "half", device: torch.device | str = "cuda"):
+        if max_positions < 1:
+            raise ValueError("max_positions must be >= 1")
+        if rotary_dim < 16 or rotary_dim % 16 != 0:
+            raise ValueError("rotary_dim must be a positive multiple of 16")
+        if pairs not in _PAIRS:
+            raise ValueError('pairs must be "half" or "interleaved"')
+        if inv_freq is None:
+            inv_freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        if tuple(inv_freq.shape) != (rotary_dim // 2,):
+            raise ValueError("inv_freq must have rotary_dim / 2 elements")
+        self.max_positions, self.rotary_dim, self.pairs = int(max_positions), int(rotary_dim), pairs
+        freq = inv_freq.detach().to(device=device, dtype=torch.float64)
+        angle = torch.arange(max_positions, device=device, dtype=torch.float64)[:, None] * freq
+        self.table = torch.stack([angle.cos().float(), angle.sin().float()], -1).contiguous()
+
+
+def _rows_ready(x: torch.Tensor) -> torch.Tensor:
+    """x itself if its rows can be read in 16-byte vectors where they lie, else a contiguous copy."""
+    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in x.stride()[:-1])
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def _view(x: torch.Tensor) -> _lib.View4:
+    if x.ndim == 4:
+        return _lib.view_bhnd(x)
+    return _lib.view4(x, rows=x.shape[1], heads=x.shape[0], batch=1, row_stride=x.stride(1), head_stride=x.stride(0))
+
+
+def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
+    if q.ndim not in (3, 4) or k.ndim != q.ndim:
+        raise ValueError("q/k must be rank-4 tensors [B, H, N, D] or packed rank-3 tensors [H, T, D]")
+    h = q.ndim - 3
+    if q.shape[:h] != k.shape[:h] or q.shape[h + 1:] != k.shape[h + 1:]:
+        raise ValueError("q and k may differ in their number of heads only")
+    if q.shape[h] < 1 or k.shape[h] < 1:
+        raise ValueError("q and k must have at least one head")
+    d = q.shape[-1]
+    validate_head_dim_supported(d)
+    _lib.dtype_code(q.dtype)
+    if k.dtype != q.dtype:
+        raise ValueError("q and k must have the same dtype")
+    if q.ndim == 3:
+        if q_meta is None:
+            raise ValueError("packed q/k need q_meta")
+        if q_meta.total_tokens != q.shape[1] or q_meta.token_indices.numel() != q.shape[1]:
+            raise ValueError("packed token count mismatch with PackMetadata")
+    elif q_meta is not None and (q_meta.B != q.shape[0] or q_meta.N != q.shape[2]):
+        raise ValueError("q_meta shape metadata does not match q/k padded shape")
+    if rotary is None and not normalize:
+        raise ValueError("nothing to do: give rotary, or normalize=True")
+    if rotary is not None and rotary.rotary_dim > d:
+        raise ValueError("rotary_dim must be at most head_dim")
+    tensors = [q, k] + ([rotary.table] if rotary is not None else [])
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if weights and not normalize:
+        raise ValueError("weights need normalize=True")
+    if any(tuple(w.shape) != (d,) for w in weights):
+        raise ValueError("q_weight and k_weight must be [head_dim]")
+    if any(w.dtype not in (torch.float32, q.dtype) or w.dtype != weights[0].dtype for w in weights):
+        raise ValueError("q_weight and k_weight must both be float32, or both of q's dtype")
+    if normalize and not eps >= 0.0:
+        raise ValueError("eps must be >= 0")
+    tensors += weights
+    if (positions is not None or position_offsets is not None) and rotary is None:
+        raise ValueError("positions need rotary")
+    if positions is not None and position_offsets is not None:
+        raise ValueError("give positions or position_offsets, not both")
+    if positions is not None:
+        want = (q.shape[1],) if q.ndim == 3 else (q.shape[0], q.shape[2])
+        if positions.dtype != torch.int32 or tuple(positions.shape) != want:
+            raise ValueError(f"positions must be an int32 tensor of shape {list(want)}")
+        tensors.append(positions)
+    if position_offsets is not None:
+        b = q_meta.B if q.ndim == 3 else q.shape[0]
+        if position_offsets.dtype != torch.int32 or tuple(position_offsets.shape) != (b,):
+            raise ValueError("position_offsets must be an int32 tensor of shape [B]")
+        tensors.append(position_offsets)
+    if q_meta is not None:
+        tensors += [q_meta.lengths, q_meta.token_indices]
+        if q_meta.lengths.dtype != torch.int32 or q_meta.token_indices.dtype != torch.int64:
+            raise ValueError("q_meta must hold int32 lengths and int64 token_indices")
+    require_cuda_tensors(*tensors)
+    if any(x.device != q.device for x in tensors):
+        raise ValueError("all tensors must be on q's device")
+
+
+def _args(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
+    """The argument block of a call, and the tensors it points into."""
+    a = _lib.QkRopeArgs()
+    packed = q.ndim == 3
+    a.dtype, a.head_dim, a.packed = _lib.dtype_code(q.dtype), q.shape[-1], int(packed)
+    a.batch, a.seq_len = (q_meta.B, max(q_meta.N, 1)) if packed else (q.shape[0], q.shape[2])
+    a.q_heads, a.k_heads = q.shape[-3], k.shape[-3]
+    a.normalize, a.eps = int(normalize), float(eps)
+    a.q, a.k = _view(q), _view(k)
+    keep = [q, k]
+
+    def ptr(x, dtype=None):
+        if x is None:
+            return None
+        x = x.detach().contiguous()
+        keep.append(x)
+        return x.data_ptr()
+
+    w = q_weight if q_weight is not None else k_weight
+    a.weight_f32 = int(w is None or w.dtype == torch.float32)
+    a.q_weight, a.k_weight = ptr(q_weight), ptr(k_weight)
+    if rotary is not None:
+        a.rotary_dim, a.pairs, a.max_positions = rotary.rotary_dim, _PAIRS[rotary.pairs], rotary.max_positions
+        a.table = rotary.table.data_ptr()
+        a.positions, a.position_offsets = ptr(positions), ptr(position_offsets)
+    if q_meta is not None:
+        if packed:
+            a.token_indices = ptr(q_meta.token_indices)
+        else:
+            a.lengths = ptr(q_meta.lengths)
+    a.error_word = _lib.error_word(q.device).data_ptr()
+    return a, keep
+
+
+def _outputs(q, k):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
+
+
+def _forward(q, k, *call):
+    out_q, out_k = _outputs(q, k)
+    if q.numel() and k.numel():
+        a, keep = _args(_rows_ready(q), _rows_ready(k), *call)
+        a.q_out, a.k_out = out_q.data_ptr(), out_k.data_ptr()
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.lib().fmlm_qk_rope_fwd(ctypes.byref(a), _lib.stream_ptr(q.device)), "qk_norm_rope")
+        del keep
+    return out_q, out_k
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, rotary, normalize, eps, q_meta, positions, position_offsets):
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, position_offsets)
+        ctx.call = (rotary, normalize, eps, q_meta)
+        return _forward(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, positions, position_offsets = ctx.saved_tensors
+        rotary, normalize, eps, q_meta = ctx.call
+        dq, dk = _outputs(q, k)
+        dwq, dwk = (torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and need else None
+                    for w, need in ((q_weight, ctx.needs_input_grad[2]), (k_weight, ctx.needs_input_grad[3])))
+        if not (q.numel() and k.numel()):
+            for w in (dwq, dwk):
+                if w is not None:
+                    w.zero_()
+            return dq, dk, dwq, dwk, None, None, None, None, None, None
+        a, keep = _args(_rows_ready(q), _rows_ready(k), rotary, q_weight, k_weight, normalize, eps, q_meta, positions,
+                        position_offsets)
+        gq, gk = _rows_ready(gq), _rows_ready(gk)
+        a.gq, a.gk = _view(gq), _view(gk)
+        a.q_out, a.k_out = dq.data_ptr(), dk.data_ptr()
+        if dwq is not None or dwk is not None:
+            a.dq_weight, a.dk_weight = (None if w is None else w.data_ptr() for w in (dwq, dwk))
+            nbytes = _lib.lib().fmlm_qk_rope_bwd_workspace_bytes(q.shape[-1])
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+        with torch.cuda.device(q.device):
+            _lib.check(_lib.lib().fmlm_qk_rope_bwd(ctypes.byref(a), _lib.stream_ptr(q.device)), "qk_norm_rope backward")
+        del keep
+        return dq, dk, dwq, dwk, None, None, None, None, None, None
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    rotary: RotaryTable | None = None,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    normalize: bool = True,
+    eps: float = 1e-6,
+    q_meta: PackMetadata | None = None,
+    positions: torch.Tensor | None = None,
+    position_offsets: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm each head row of q and k and rotate it by its position, in one pass.
+
+    q [B, H, N, D] (dense, or padded with ``q_meta``: rows past a sequence come
+    out as zeros, whatever they hold) or packed [H, T, D] with ``q_meta``; k the
+    same with any number of heads.  Any strides, a projection's [B, N, H, D]
+    transposed among them.
+
+    ``normalize``: x / sqrt(mean(x^2) + eps) over the head dimension, times
+    ``q_weight`` / ``k_weight`` [D] (float32 or q's dtype; None: ones).
+    ``rotary`` (None: no rotation): the token's index in its sequence is its
+    position, plus ``position_offsets[b]`` (int32 [B]: tokens that came before,
+    as a cached context's), or ``positions`` (int32 [B, N], packed [T]) gives
+    it.  A position outside the table uses the table's nearest row and sets
+    the error word (``check_device_errors``).
+
+    Returns the new q and k, contiguous, in the layouts and dtype they came in.
+    Differentiable in q, k, q_weight and k_weight.
+    """
+    _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, rotary, normalize, eps, q_meta, positions, position_offsets)
+    return _forward(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)

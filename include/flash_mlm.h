@@ -196,6 +196,50 @@ FMLM_API int fmlm_attn_bwd(const fmlm_attn_bwd_args* args, void* stream);
 /* Workspace for fmlm_attn_bwd; rows = output rows (B*H*N dense or padded, H*T packed). */
 FMLM_API size_t fmlm_attn_bwd_workspace_bytes(int64_t rows);
 
+enum { FMLM_PAIRS_HALF = 0, FMLM_PAIRS_INTERLEAVED = 1 };
+
+/* Arguments of the per-head norm with position rotation (no counterpart in the
+ * reference).  For every head row x of q and k:
+ *   n = x / sqrt(mean(x^2) + eps) * weight        (normalize; else n = x)
+ *   y = n with its first rotary_dim columns rotated by the row's position:
+ *       pair j = columns (j, j + rotary_dim / 2) (halves) or (2j, 2j + 1)
+ *       (interleaved), turned by the angle whose cosine and sine are
+ *       table[position][j]. */
+typedef struct fmlm_qk_rope_args {
+  int32_t dtype, head_dim;        /* FMLM_DTYPE_*; 16, 32, 64, 128, 256 */
+  int32_t packed;                 /* 0: q, k are [B][heads][N][D]; 1: [heads][T][D] (views of batch 1, rows T) */
+  int32_t batch, seq_len;         /* B, N (packed: N of token_indices) */
+  int32_t q_heads, k_heads;
+  int32_t normalize;
+  int32_t weight_f32;             /* 1: weights (and their gradients) are float32; 0: q's dtype */
+  int32_t rotary_dim;             /* 0: no rotation; else a multiple of 16, at most head_dim */
+  int32_t pairs;                  /* FMLM_PAIRS_* */
+  int32_t max_positions;          /* rows of table */
+  float eps;
+  fmlm_view4 q, k;                /* any strides (multiples of 8 elements, 16-byte aligned base), innermost 1 */
+  fmlm_view4 gq, gk;              /* backward: gradients of the outputs, like q, k */
+  const void *q_weight, *k_weight;/* [head_dim] or NULL (ones) */
+  const float* table;             /* [max_positions][rotary_dim / 2][2] cosine, sine */
+  const int32_t* positions;       /* optional, one per token ([B][N] or [T]); else the token's index in its
+                                     sequence, plus position_offsets[b] where given */
+  const int32_t* position_offsets;/* optional [B] */
+  const int32_t* lengths;         /* optional [B] (not packed): rows past them come out as zeros, unread */
+  const int64_t* token_indices;   /* packed: b * N + n of every token */
+  void *q_out, *k_out;            /* contiguous: outputs, or (backward) the gradients of q, k */
+  void *dq_weight, *dk_weight;    /* backward, optional: gradients of the weights */
+  void* workspace;                /* backward: fmlm_qk_rope_bwd_workspace_bytes() bytes */
+  size_t workspace_bytes;
+  int32_t* error_word;            /* set to 6 if a position lies outside the table (the nearest row is used) */
+} fmlm_qk_rope_args;
+
+FMLM_API int fmlm_qk_rope_fwd(const fmlm_qk_rope_args* args, void* stream);
+
+/* Gradients of q, k and the weights from gq, gk (q, k and the rest as in the
+ * forward call).  The weights' sums are taken in a fixed order: the same
+ * inputs give the same bits. */
+FMLM_API int fmlm_qk_rope_bwd(const fmlm_qk_rope_args* args, void* stream);
+FMLM_API size_t fmlm_qk_rope_bwd_workspace_bytes(int32_t head_dim);
+
 /* Gather the valid rows of x [B][H][N][D] into out [H * total_padded, D], zeroing
  * rows [total_tokens, total_padded) of every head.
  * Replaces _pack_flatten_for_kernel_into / pack_for_kernel
