@@ -18,9 +18,9 @@
 // registers in the layout in which the tensor cores read A from TMEM, as in
 // the Q pass; P and dS never touch shared memory.
 //
-// Roles of a persistent CTA (one per SM): warps 0-7 do the element-wise work
-// (warp w: TMEM lanes 32 (w % 4) .., column half w / 4 of every score tile),
-// warp 8 loads tiles by TMA and decodes work items, warp 9 issues the MMAs.
+// Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
+// (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
+// warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -63,15 +63,24 @@ struct BwdCfg {
   static constexpr int NSLAB = D / SLAB_COLS;
   static constexpr int A_BYTES = BM * D * 2;
   static constexpr int B_BYTES = BN * D * 2;
-  static constexpr int ABUF = D <= 64 ? 2 : 1;
   static constexpr int STAGES = D <= 64 ? 4 : D == 128 ? 2 : 1;
-  static constexpr int EW_WARPS = 8;
+  // The stationary tiles as A operands in TMEM, where there is room: with both
+  // operands in shared memory an MMA of 128 x 128 x 16 reads 8 KB in 64 cycles,
+  // all that shared memory delivers, and every barrier and load waits behind it.
+  static constexpr bool ATM = KV ? D <= 64 : D <= 128;
+  static constexpr int ABUF = D <= 64 ? 2 : 1;
+  // P in columns of its own (KV): the next S need not wait until P is consumed.
+  static constexpr bool SEP_P = KV && D <= 64;
+  static constexpr int EW_GROUPS = 4;
+  static constexpr int EW_WARPS = 4 * EW_GROUPS;
   static constexpr int TMA_WARP = EW_WARPS;
   static constexpr int MMA_WARP = EW_WARPS + 1;
   static constexpr int THREADS = 32 * (EW_WARPS + 2);
-  static constexpr int NC = BN / 2;  // score columns per element-wise warp
-  static constexpr int TM_S = 0, TM_DP = BN, TM_ACC1 = 2 * BN, TM_ACC2 = 2 * BN + (KV ? DV : 0);
-  static constexpr int TMEM_USED = TM_ACC2 + DV;
+  static constexpr int NC = BN / EW_GROUPS;  // score columns per element-wise warp
+  static constexpr int TM_S = 0, TM_DP = BN, TM_P = SEP_P ? 2 * BN : 0;
+  static constexpr int TM_ACC1 = 2 * BN + (SEP_P ? BN / 2 : 0), TM_ACC2 = TM_ACC1 + (KV ? DV : 0);
+  static constexpr int TM_A1 = TM_ACC2 + DV, TM_A2 = TM_A1 + (ATM ? D / 2 : 0);
+  static constexpr int TMEM_USED = TM_A2 + (ATM ? D / 2 : 0);
   static_assert(TMEM_USED <= 512, "TMEM budget");
   static constexpr int TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
   static constexpr int STAT_BYTES = KV ? STAGES * BN * 8 : 0;
@@ -191,8 +200,11 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
 struct __align__(8) BwdBarriers {
   uint64_t a_full[2], a_empty[2];
   uint64_t b1_full[4], b2_full[4], b1_empty[4], b2_empty[4];
-  uint64_t s_full, dp_full;  // MMA -> element-wise: S / dP complete
-  uint64_t p_full, ds_full;  // element-wise -> MMA: P written (Q pass: S read) / dS written
+  uint64_t a_tm;              // element-wise -> MMA: the stationary tiles are in TMEM
+  uint64_t s_full, dp_full;   // MMA -> element-wise: S / dP complete
+  uint64_t s_free;            // element-wise -> MMA: S is in registers
+  uint64_t p_full, ds_full;   // element-wise -> MMA: P / dS written
+  uint64_t p_free;            // MMA -> element-wise (separate P): P consumed
   uint64_t acc_full, acc_empty;
   uint64_t item_full[4], item_empty[4];
   int item_idx[4];
@@ -208,6 +220,36 @@ struct BwdScale {
   static constexpr float kPExp = BF16 ? 0.f : 12.f;
   static constexpr float kInv = BF16 ? 1.f : 1.f / 4096.f;
 };
+
+// MMA issue with the shared-memory descriptors as (low word, constant high
+// word): the low word holds the address, so stepping through a tile is one
+// 32-bit add and the high words never leave their registers.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tm, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tm), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// 16-byte vector c of row r of a K-major tile as TMA's swizzle laid it out.
+template <int SWB>
+__device__ __forceinline__ uint4 ld_swizzled(const uint8_t* tile, int rows, int r, int c) {
+  constexpr int V = SWB / 16;  // vectors per row of a slab
+  const int x = ((r * SWB) >> 7) & (V - 1);
+  return *reinterpret_cast<const uint4*>(tile + (c / V) * (rows * SWB) + r * SWB + (((c % V) ^ x) << 4));
+}
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -228,7 +270,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
                     const BwdParams p) {
   using C = BwdCfg<D, KV>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  constexpr int BN = C::BN, SWB = C::SWB, STAGES = C::STAGES, NC = C::NC;
+  constexpr int BN = C::BN, SWB = C::SWB, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;                            // [ABUF][A1, A2]
@@ -244,7 +286,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->a_full[i], 1);
-      mbar_init(&bar->a_empty[i], 1);
+      mbar_init(&bar->a_empty[i], C::ATM ? C::EW_WARPS : 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&bar->b1_full[i], KV ? 2 : 1);  // KV: the tile, and its rows' stats
@@ -256,6 +298,9 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     }
     mbar_init(&bar->s_full, 1);
     mbar_init(&bar->dp_full, 1);
+    mbar_init(&bar->a_tm, C::EW_WARPS);
+    mbar_init(&bar->s_free, C::EW_WARPS);
+    mbar_init(&bar->p_free, 1);
     mbar_init(&bar->p_full, C::EW_WARPS);
     mbar_init(&bar->ds_full, C::EW_WARPS);
     mbar_init(&bar->acc_full, 1);
@@ -292,13 +337,15 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     failed = __any_sync(0xffffffffu, failed);
     return !failed;
   };
-  auto take_item = [&](uint32_t ring, BwdItem& it) -> bool {
-    if (failed || !wait(&bar->item_full[ring & 3], (ring >> 2) & 1u)) return false;
+  // The next published item, in its ring slot until release_item; nullptr: no more.
+  auto take_item = [&](uint32_t ring) -> const BwdItem* {
+    if (failed || !wait(&bar->item_full[ring & 3], (ring >> 2) & 1u)) return nullptr;
     const int w = *reinterpret_cast<volatile int*>(&bar->item_idx[ring & 3]);
-    if (w < num_items) it = ring_items[ring & 3];
+    return w < num_items ? ring_items + (ring & 3) : nullptr;
+  };
+  auto release_item = [&](uint32_t ring) {
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar->item_empty[ring & 3]);
-    return w < num_items;
   };
 
   if (warp == C::TMA_WARP) {
@@ -308,9 +355,18 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     auto load_tile = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* b, int rows, int row, int h, int bb) {
       for (int s = 0; s < C::NSLAB; ++s) tma_load_4d(dst + s * (rows * SWB), m, b, s * C::SLAB_COLS, row, h, bb);
     };
+    auto next_item = [&]() {
+      int next = 0;
+      if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
+      w = __shfl_sync(0xffffffffu, next, 0);
+    };
     for (uint32_t ring = 0;; ++ring) {
       BwdItem it;
-      if (w < num_items) it = decode_bwd_item<C>(p, w, lane);
+      while (w < num_items) {
+        it = decode_bwd_item<C>(p, w, lane);
+        if (it.limit > 0) break;  // (a slot past its sequence's end writes nothing)
+        next_item();
+      }
       if (!wait(&bar->item_empty[ring & 3], ((ring >> 2) & 1u) ^ 1u)) break;
       if (lane == 0) {
         if (w < num_items) ring_items[ring & 3] = it;
@@ -372,9 +428,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         }
         if (failed) break;
       }
-      int next = 0;
-      if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
-      w = __shfl_sync(0xffffffffu, next, 0);
+      next_item();
     }
   } else if (warp == C::MMA_WARP) {
     // ------------------------------------------------------------ MMA issuer
@@ -384,34 +438,39 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     constexpr uint32_t layout = swizzle_code(SWB);
     const uint32_t sA0 = smem_u32(sA), sB0 = smem_u32(sB);
     const bool leader = elect_one();
-    uint32_t fill = 0, aload = 0, p_ph = 0, ds_ph = 0, acc_ph = 1;
-    // scores: D[128, BN] = A[128, D] B[BN, D]^T
-    auto issue_scores = [&](uint32_t d, uint32_t a_base, uint32_t b_base) {
+    // high descriptor word: 8-row stride, descriptor version 1, swizzle
+    constexpr uint32_t hi = (8 * SWB >> 4) | (1u << 14) | (layout << 29);
+    constexpr uint32_t lbo_k = 1u << 16;                // K-major: unused
+    constexpr uint32_t lbo_mn = (BN * SWB >> 4) << 16;  // MN-major: slab stride
+    // scores: D[128, BN] = A[128, D] B[BN, D]^T (A in TMEM or shared memory), then commit to `done`
+    auto issue_scores = [&](uint32_t d, uint32_t a_tm, uint32_t a_base, uint32_t b_base, uint64_t* done) {
       if (leader) {
+        const uint32_t a = (a_base >> 4) | lbo_k, b = (b_base >> 4) | lbo_k;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t slab = (kk * 32) / SWB, inrow = (kk * 32) % SWB;
-          umma_ss(d, make_smem_desc(a_base + slab * (C::BM * SWB) + inrow, 16, 8 * SWB, layout),
-                  make_smem_desc(b_base + slab * (BN * SWB) + inrow, 16, 8 * SWB, layout), idesc_s, kk > 0 ? 1u : 0u);
+          const uint32_t bk = b + ((slab * (BN * SWB) + inrow) >> 4);
+          if constexpr (C::ATM) mma_ts(d, a_tm + kk * 8, bk, hi, idesc_s, kk > 0 ? 1u : 0u);
+          else mma_ss(d, a + ((slab * (C::BM * SWB) + inrow) >> 4), bk, hi, idesc_s, kk > 0 ? 1u : 0u);
         }
+        umma_commit(done);
       }
     };
-    // accumulators: D[128, DV] += A[128, BN] (16-bit, TMEM) B[BN, DV]; each
-    // column half of A lies at the start of that half of the score tile.
-    auto issue_acc = [&](uint32_t d, uint32_t a_tm, uint32_t b_base, bool acc) {
+    // accumulators: D[128, DV] += A[128, BN] (16-bit, TMEM) B[BN, DV].  A's
+    // columns are in EW_GROUPS pieces, `piece` TMEM columns apart.
+    auto issue_acc = [&](uint32_t d, uint32_t a_tm, uint32_t piece, uint32_t b_base, bool acc, uint64_t* done) {
       if (leader) {
+        constexpr int KP = C::NC / 16;  // K steps per piece
+        const uint32_t b = (b_base >> 4) | lbo_mn;
+        mma_ts(d, a_tm, b, hi, idesc_acc, acc ? 1u : 0u);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          constexpr int HK = BN / 32;  // K steps per half
-          const uint32_t a = a_tm + (kk / HK) * (BN / 2) + (kk % HK) * 8;
-          umma_ts(d, a, make_smem_desc(b_base + kk * 16 * SWB, BN * SWB, 8 * SWB, layout), idesc_acc,
-                  (acc || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 1; kk < BN / 16; ++kk)
+          mma_ts(d, a_tm + (kk / KP) * piece + (kk % KP) * 8, b + (kk * 16 * SWB >> 4), hi, idesc_acc, 1u);
+        umma_commit(done);
       }
     };
     auto commit = [&](uint64_t* b) {
       if (leader) umma_commit(b);
-      __syncwarp();
     };
     // Rows past the range hold another sequence's rows or padding, NaN perhaps:
     // P and dS are 0 there, but 0 * NaN is not.
@@ -425,67 +484,76 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         __syncwarp();
       }
     };
-    BwdItem it;
-    for (uint32_t ring = 0; take_item(ring, it); ++ring) {
-      const int n = it.heads * it.nt0 + it.nt1;
+    uint32_t fill = 0, aload = 0, ph = 0, acc_ph = 1;
+    for (uint32_t ring = 0;; ++ring) {
+      const BwdItem* slot = take_item(ring);
+      if (!slot) break;
+      const int dh = slot->dh, nt0 = slot->nt0, row0 = slot->row0, end0 = slot->end0, row1 = slot->row1,
+                end1 = slot->end1, n = slot->heads * nt0 + slot->nt1;
+      release_item(ring);
       if (n == 0) continue;
       const int ab = aload % C::ABUF;
-      if (!wait(&bar->a_full[ab], (aload / C::ABUF) & 1u)) break;
+      if (!wait(C::ATM ? &bar->a_tm : &bar->a_full[ab], C::ATM ? (aload & 1u) : (aload / C::ABUF) & 1u)) break;
       ++aload;
       const uint32_t a1 = sA0 + ab * 2 * C::A_BYTES, a2 = a1 + C::A_BYTES;
-      const uint32_t dh_off = (it.dh * C::DV / C::SLAB_COLS) * (BN * SWB);
-      // valid rows of streamed tile i; tiles are asked for in order, each twice (S, dP)
-      auto valid_rows = [&](int i) {
-        int t = KV ? i % it.nt0 : i;
-        if (!KV && t >= it.nt0) return it.end1 - (it.row1 + (t - it.nt0) * BN);
-        return it.end0 - (it.row0 + t * BN);
+      const uint32_t dh_off = (dh * C::DV / C::SLAB_COLS) * (BN * SWB);
+      // Tiles are asked for in order: S and dP each keep the tile's place in its range.
+      auto valid_rows = [&](int t) {
+        return (!KV && t >= nt0) ? end1 - (row1 + (t - nt0) * BN) : end0 - (row0 + t * BN);
       };
+      int ts = 0, td = 0;
       auto do_s = [&](int i) -> bool {
         const uint32_t f = fill + i;
         const int st = f % STAGES;
         if (!wait(&bar->b1_full[st], (f / STAGES) & 1u)) return false;
-        clear_rows(sB + st * 2 * C::B_BYTES, valid_rows(i));
+        clear_rows(sB + st * 2 * C::B_BYTES, valid_rows(ts));
+        if (++ts == nt0 && KV) ts = 0;
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_S, a1, sB0 + st * 2 * C::B_BYTES);
-        commit(&bar->s_full);
+        issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + st * 2 * C::B_BYTES, &bar->s_full);
         return true;
       };
       auto do_dp = [&](int i) -> bool {
         const uint32_t f = fill + i;
         const int st = f % STAGES;
         if (!wait(&bar->b2_full[st], (f / STAGES) & 1u)) return false;
-        clear_rows(sB + st * 2 * C::B_BYTES + C::B_BYTES, valid_rows(i));
+        clear_rows(sB + st * 2 * C::B_BYTES + C::B_BYTES, valid_rows(td));
+        if (++td == nt0 && KV) td = 0;
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_DP, a2, sB0 + st * 2 * C::B_BYTES + C::B_BYTES);
-        commit(&bar->dp_full);
+        issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + st * 2 * C::B_BYTES + C::B_BYTES, &bar->dp_full);
         if (!KV) commit(&bar->b2_empty[st]);
-        if (i + 1 == n) commit(&bar->a_empty[ab]);
+        if (!C::ATM && i + 1 == n) commit(&bar->a_empty[ab]);
         return true;
       };
       if (!do_s(0) || !do_dp(0)) break;
       bool ok = true;
-      for (int i = 0; i < n && ok; ++i) {
+      for (int i = 0; i < n && ok; ++i, ph ^= 1u) {
         const int st = (fill + i) % STAGES;
         const uint32_t b1 = sB0 + st * 2 * C::B_BYTES, b2 = b1 + C::B_BYTES;
-        if (!wait(&bar->p_full, p_ph)) { ok = false; break; }
-        p_ph ^= 1u;
+        // S(i+1) as soon as its columns are free: S(i) is in registers, and
+        // (KV, P over S) P(i) is consumed, the MMAs running in order.  One
+        // stage only: its tile B1 takes the place of the one dS(i) still needs.
+        constexpr bool kEarlyS = C::SEP_P || !KV;
+        if (kEarlyS && STAGES > 1) {
+          if (!wait(&bar->s_free, ph)) { ok = false; break; }
+          if (i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+        }
+        if constexpr (KV) {
+          if (!wait(&bar->p_full, ph)) { ok = false; break; }
+        }
         if (i == 0) {
           if (!wait(&bar->acc_empty, acc_ph)) { ok = false; break; }
           acc_ph ^= 1u;
         }
-        tc_fence_after();
         if constexpr (KV) {
-          issue_acc(tmem_base + C::TM_ACC1, tmem_base + C::TM_S, b2 + dh_off, i > 0);
-          commit(&bar->b2_empty[st]);
+          tc_fence_after();
+          issue_acc(tmem_base + C::TM_ACC1, tmem_base + C::TM_P, C::SEP_P ? C::NC / 2 : C::NC, b2 + dh_off, i > 0,
+                    &bar->b2_empty[st]);
+          if (C::SEP_P) commit(&bar->p_free);
         }
-        // S(i+1) runs while the element-wise warps turn dP(i) into dS(i).  One
-        // stage only: its tile B1 takes the place of the one dS(i) still needs.
-        if (STAGES > 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
-        if (!wait(&bar->ds_full, ds_ph)) { ok = false; break; }
-        ds_ph ^= 1u;
+        if (!kEarlyS && STAGES > 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+        if (!wait(&bar->ds_full, ph)) { ok = false; break; }
         tc_fence_after();
-        issue_acc(tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, b1 + dh_off, i > 0);
-        commit(&bar->b1_empty[st]);
+        issue_acc(tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1 + dh_off, i > 0, &bar->b1_empty[st]);
         if (i + 1 == n) commit(&bar->acc_full);
         if (STAGES == 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
         if (i + 1 < n && !do_dp(i + 1)) { ok = false; break; }
@@ -498,113 +566,144 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const int g = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    constexpr int NC = C::NC;
     const uint32_t tS = tmem_base + lane_off + C::TM_S + g * NC;
     const uint32_t tDP = tmem_base + lane_off + C::TM_DP + g * NC;
+    const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
     const float sl2 = p.scale_log2;
     constexpr float kInv = BwdScale<BF16>::kInv;
-    uint32_t fill = 0, ph = 0, acc_ph = 0;
+    uint32_t fill = 0, ph = 0, acc_ph = 0, aload = 0;
     auto arrive = [&](uint64_t* b) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
-    BwdItem it;
-    for (uint32_t ring = 0; take_item(ring, it); ++ring) {
-      const int n = it.heads * it.nt0 + it.nt1;
+    auto ld = [&](uint32_t a, uint32_t(&r)[NC]) {
+      if constexpr (NC == 32) tmem_ld_x32(a, r); else tmem_ld_x16(a, r);
+    };
+    auto st16 = [&](uint32_t a, const uint32_t(&r)[NC / 2]) {
+      if constexpr (NC == 32) tmem_st_x16_nowait(a, r); else tmem_st_x8_nowait(a, r);
+      tmem_wait_st();
+    };
+    // Stationary tiles, shared memory -> TMEM: half the warps copy A1, half A2,
+    // (D > 16) each warp half of its rows' columns.
+    auto copy_a = [&]() -> bool {
+      const int ab = aload % C::ABUF;
+      if (!wait(&bar->a_full[ab], (aload / C::ABUF) & 1u)) return false;
+      ++aload;
+      constexpr int W = D > 16 ? D / 4 : 8;  // 32-bit words per thread
+      const int half = D > 16 ? g & 1 : 0;
+      if (D > 16 || (g & 1) == 0) {
+        const uint8_t* tile = sA + ab * 2 * C::A_BYTES + (g >> 1) * C::A_BYTES;
+        uint32_t v[W];
+#pragma unroll
+        for (int c = 0; c < W / 4; ++c) {
+          const uint4 x = ld_swizzled<SWB>(tile, C::BM, row, half * (W / 4) + c);
+          v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
+        }
+        const uint32_t dst = tmem_base + lane_off + ((g >> 1) ? C::TM_A2 : C::TM_A1) + half * W;
+        if constexpr (W == 64) tmem_st_x64(dst, v);
+        else if constexpr (W == 32) tmem_st_x32(dst, v);
+        else if constexpr (W == 16) tmem_st_x16(dst, v);
+        else tmem_st_x8(dst, v);
+      }
+      arrive(&bar->a_tm);
+      if (lane == 0) mbar_arrive(&bar->a_empty[ab]);
+      return true;
+    };
+    const BwdItem* it = take_item(0);
+    if (C::ATM && it && it->heads * it->nt0 + it->nt1 > 0 && !copy_a()) it = nullptr;
+    for (uint32_t ring = 0; it; ++ring) {
+      const int nt0 = it->nt0, n = it->heads * nt0 + it->nt1;
       float2 rs = make_float2(0.f, 0.f);
-      if (!KV && row < it.valid) rs = __ldg(p.stats + it.out_row + row);
-      for (int i = 0; i < n; ++i, ++fill) {
+      if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
+      for (int i = 0; i < n; ++i, ++fill, ph ^= 1u) {
         const int stg = fill % STAGES;
         const float* ss = sStat + stg * 2 * BN + g * NC;
         if (KV && !wait(&bar->b1_full[stg], (fill / STAGES) & 1u)) break;
         if (!wait(&bar->s_full, ph)) break;
         tc_fence_after();
-        // Columns in chunks of 32, each stored as soon as it is packed: P stays
-        // in registers for dS, so the budget (168: three warps share a quarter
-        // of the register file) leaves room for one chunk of scores beside it.
+        uint32_t x[NC];
         float pr[NC];
-#pragma unroll
-        for (int h = 0; h < NC; h += 32) {
-          uint32_t x[32];
-          tmem_ld_x32(tS + h, x);
-          if constexpr (KV) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 nl = *reinterpret_cast<const float4*>(ss + h + c);
-              pr[h + c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, nl.x));
-              pr[h + c + 1] = ex2_approx(fmaf(__uint_as_float(x[c + 1]), sl2, nl.y));
-              pr[h + c + 2] = ex2_approx(fmaf(__uint_as_float(x[c + 2]), sl2, nl.z));
-              pr[h + c + 3] = ex2_approx(fmaf(__uint_as_float(x[c + 3]), sl2, nl.w));
-            }
-            uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) pk[c] = pack2<BF16>(pr[h + 2 * c], pr[h + 2 * c + 1]);
-            tmem_st_x16_nowait(tS + h / 2, pk);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) pr[h + c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, rs.x));
-          }
-        }
+        ld(tS, x);
+        if (C::SEP_P || !KV) arrive(&bar->s_free);
         if constexpr (KV) {
-          tmem_wait_st();
+#pragma unroll
+          for (int c = 0; c < NC; c += 4) {
+            const float4 nl = *reinterpret_cast<const float4*>(ss + c);
+            pr[c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, nl.x));
+            pr[c + 1] = ex2_approx(fmaf(__uint_as_float(x[c + 1]), sl2, nl.y));
+            pr[c + 2] = ex2_approx(fmaf(__uint_as_float(x[c + 2]), sl2, nl.z));
+            pr[c + 3] = ex2_approx(fmaf(__uint_as_float(x[c + 3]), sl2, nl.w));
+          }
+          uint32_t pk[NC / 2];
+#pragma unroll
+          for (int c = 0; c < NC / 2; ++c) pk[c] = pack2<BF16>(pr[2 * c], pr[2 * c + 1]);
+          if (C::SEP_P) {
+            if (!wait(&bar->p_free, ph ^ 1u)) break;
+            tc_fence_after();
+          }
+          st16(tP, pk);
+          arrive(&bar->p_full);
         } else {
-          const bool second = i >= it.nt0;
-          const int valid = (second ? it.end1 - (it.row1 + (i - it.nt0) * BN) : it.end0 - (it.row0 + i * BN)) - g * NC;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) pr[c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, rs.x));
+          const int valid = (i >= nt0 ? it->end1 - (it->row1 + (i - nt0) * BN) : it->end0 - (it->row0 + i * BN)) - g * NC;
           if (valid < NC) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
               if (c >= valid) pr[c] = 0.f;
           }
         }
-        arrive(&bar->p_full);  // KV: P is written.  Q: S is read
         if (!wait(&bar->dp_full, ph)) break;
         tc_fence_after();
-        ph ^= 1u;
+        ld(tDP, x);
+        uint32_t pk[NC / 2];
 #pragma unroll
-        for (int h = 0; h < NC; h += 32) {
-          uint32_t x[32], pk[16];
-          tmem_ld_x32(tDP + h, x);
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            float4 nd;
-            if constexpr (KV) nd = *reinterpret_cast<const float4*>(ss + BN + h + c);
-            else nd = make_float4(rs.y, rs.y, rs.y, rs.y);
-            pk[c / 2] = pack2<BF16>(pr[h + c] * fmaf(__uint_as_float(x[c]), kInv, nd.x),
-                                    pr[h + c + 1] * fmaf(__uint_as_float(x[c + 1]), kInv, nd.y));
-            pk[c / 2 + 1] = pack2<BF16>(pr[h + c + 2] * fmaf(__uint_as_float(x[c + 2]), kInv, nd.z),
-                                        pr[h + c + 3] * fmaf(__uint_as_float(x[c + 3]), kInv, nd.w));
-          }
-          tmem_st_x16_nowait(tDP + h / 2, pk);
+        for (int c = 0; c < NC; c += 4) {
+          float4 nd;
+          if constexpr (KV) nd = *reinterpret_cast<const float4*>(ss + BN + c);
+          else nd = make_float4(rs.y, rs.y, rs.y, rs.y);
+          pk[c / 2] = pack2<BF16>(pr[c] * fmaf(__uint_as_float(x[c]), kInv, nd.x),
+                                  pr[c + 1] * fmaf(__uint_as_float(x[c + 1]), kInv, nd.y));
+          pk[c / 2 + 1] = pack2<BF16>(pr[c + 2] * fmaf(__uint_as_float(x[c + 2]), kInv, nd.z),
+                                      pr[c + 3] * fmaf(__uint_as_float(x[c + 3]), kInv, nd.w));
         }
-        tmem_wait_st();
+        st16(tDP, pk);
         arrive(&bar->ds_full);
       }
       if (failed) break;
-      // epilogue: accumulators -> global.  KV: warps 0-3 dV, 4-7 dK; Q: the two halves of dQ's columns
       if (n > 0) {
         if (!wait(&bar->acc_full, acc_ph)) break;
         acc_ph ^= 1u;
         tc_fence_after();
       }
-      constexpr int COLS = KV ? C::DV : (D >= 32 ? D / 2 : D);  // columns per warp
-      constexpr int OC = COLS >= 32 ? 32 : 16;
-      const bool mine = KV || D >= 32 || g == 0;
-      if (mine) {
-        const uint32_t tO = tmem_base + lane_off + (KV ? (g == 0 ? C::TM_ACC1 : C::TM_ACC2) : C::TM_ACC2 + g * COLS);
-        const float f = KV && g == 0 ? kInv : p.scale;
-        T* base = reinterpret_cast<T*>(KV ? (g == 0 ? (it.a_map ? p.dvc : p.dv) : (it.a_map ? p.dkc : p.dk)) : p.dq);
-        T* dst = base + (it.out_row + row) * (long long)D + (KV ? it.dh * C::DV : g * COLS);
+      // Every MMA of this item is done, so the next item's stationary tiles
+      // can move in before the epilogue: its first scores run during it.
+      const BwdItem* next = take_item(ring + 1);
+      if (failed) break;
+      if (C::ATM && next && next->heads * next->nt0 + next->nt1 > 0 && !copy_a()) break;
+      // epilogue: accumulators -> global, a quarter of the columns per warp group
+      // (KV: groups 0, 1 halves of dV, groups 2, 3 halves of dK)
+      constexpr int PARTS = KV ? 2 : 4;
+      constexpr int COLS = C::DV / PARTS >= 16 ? C::DV / PARTS : 16;
+      const int part = KV ? g & 1 : g;
+      if (part * COLS < C::DV) {
+        const bool is_dv = KV && g < 2;
+        const uint32_t tO = tmem_base + lane_off + (is_dv ? C::TM_ACC1 : C::TM_ACC2) + part * COLS;
+        const float f = is_dv ? kInv : p.scale;
+        const int valid = it->valid, limit = it->limit;
+        T* base = reinterpret_cast<T*>(!KV ? p.dq : is_dv ? (it->a_map ? p.dvc : p.dv) : (it->a_map ? p.dkc : p.dk));
+        T* dst = base + (it->out_row + row) * (long long)D + it->dh * C::DV + part * COLS;
 #pragma unroll 1
-        for (int c0 = 0; c0 < COLS; c0 += OC) {
-          uint32_t o[OC];
-          if (n > 0) {
-            if constexpr (OC == 32) tmem_ld_x32(tO + c0, o); else tmem_ld_x16(tO + c0, o);
-          }
-          if (row < it.limit) {
-            const bool live = n > 0 && row < it.valid;
+        for (int c0 = 0; c0 < COLS; c0 += 16) {
+          uint32_t o[16];
+          if (n > 0) tmem_ld_x16(tO + c0, o);
+          if (row < limit) {
+            const bool live = n > 0 && row < valid;
             uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
 #pragma unroll
-            for (int q = 0; q < OC / 8; ++q) {
+            for (int q = 0; q < 2; ++q) {
               uint32_t v[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -616,6 +715,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         }
       }
       if (n > 0) arrive(&bar->acc_empty);
+      release_item(ring);
+      it = next;
     }
   }
 
