@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   };
   // Whole-warp wait; false once anything in the CTA has given up.
   auto wait = [&](uint64_t* b, uint32_t ph) -> bool {
+    if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(b), ph))) return true;
     if (!mbar_wait(b, ph, abort_flag, tmo)) fail();
     failed = __any_sync(0xffffffffu, failed);
     return !failed;
@@ -484,82 +485,98 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         __syncwarp();
       }
     };
-    uint32_t fill = 0, aload = 0, ph = 0, acc_ph = 1;
+    // Everything below is kept incremental (stage, phase, tiles left in the
+    // range): between two MMA batches this warp's own instructions are on the
+    // critical path.
+    struct Stage {
+      uint32_t i = 0, ph = 0;
+      __device__ __forceinline__ void next() {
+        if (++i == (uint32_t)STAGES) {
+          i = 0;
+          ph ^= 1u;
+        }
+      }
+    };
+    Stage s_st, d_st, c_st;  // stages of the next S, the next dP, the current accumulations
+    uint32_t aload = 0, ph = 0, acc_ph = 1;
     for (uint32_t ring = 0;; ++ring) {
       const BwdItem* slot = take_item(ring);
       if (!slot) break;
-      const int dh = slot->dh, nt0 = slot->nt0, row0 = slot->row0, end0 = slot->end0, row1 = slot->row1,
-                end1 = slot->end1, n = slot->heads * nt0 + slot->nt1;
+      const int nt0 = slot->nt0, nt1 = slot->nt1, n = slot->heads * nt0 + nt1;
+      // valid rows of each range's last tile
+      const int last0 = slot->end0 - slot->row0 - (nt0 - 1) * BN, last1 = slot->end1 - slot->row1 - (nt1 - 1) * BN;
+      const uint32_t dh_off = (slot->dh * C::DV / C::SLAB_COLS) * (BN * SWB);
       release_item(ring);
       if (n == 0) continue;
       const int ab = aload % C::ABUF;
       if (!wait(C::ATM ? &bar->a_tm : &bar->a_full[ab], C::ATM ? (aload & 1u) : (aload / C::ABUF) & 1u)) break;
       ++aload;
       const uint32_t a1 = sA0 + ab * 2 * C::A_BYTES, a2 = a1 + C::A_BYTES;
-      const uint32_t dh_off = (dh * C::DV / C::SLAB_COLS) * (BN * SWB);
-      // Tiles are asked for in order: S and dP each keep the tile's place in its range.
-      auto valid_rows = [&](int t) {
-        return (!KV && t >= nt0) ? end1 - (row1 + (t - nt0) * BN) : end0 - (row0 + t * BN);
-      };
-      int ts = 0, td = 0;
-      auto do_s = [&](int i) -> bool {
-        const uint32_t f = fill + i;
-        const int st = f % STAGES;
-        if (!wait(&bar->b1_full[st], (f / STAGES) & 1u)) return false;
-        clear_rows(sB + st * 2 * C::B_BYTES, valid_rows(ts));
-        if (++ts == nt0 && KV) ts = 0;
+      // Tiles left in the range that S / dP walk, and that range's last tile.
+      int s_left = nt0 > 0 ? nt0 : nt1, d_left = s_left;
+      int s_last = nt0 > 0 ? last0 : last1, d_last = s_last;
+      auto do_s = [&]() -> bool {
+        if (!wait(&bar->b1_full[s_st.i], s_st.ph)) return false;
+        if (--s_left == 0) {
+          if (s_last < BN) clear_rows(sB + s_st.i * 2 * C::B_BYTES, s_last);
+          s_left = KV ? nt0 : nt1;
+          if (!KV) s_last = last1;
+        }
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + st * 2 * C::B_BYTES, &bar->s_full);
+        issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + s_st.i * 2 * C::B_BYTES, &bar->s_full);
+        s_st.next();
         return true;
       };
-      auto do_dp = [&](int i) -> bool {
-        const uint32_t f = fill + i;
-        const int st = f % STAGES;
-        if (!wait(&bar->b2_full[st], (f / STAGES) & 1u)) return false;
-        clear_rows(sB + st * 2 * C::B_BYTES + C::B_BYTES, valid_rows(td));
-        if (++td == nt0 && KV) td = 0;
+      auto do_dp = [&]() -> bool {
+        if (!wait(&bar->b2_full[d_st.i], d_st.ph)) return false;
+        if (--d_left == 0) {
+          if (d_last < BN) clear_rows(sB + d_st.i * 2 * C::B_BYTES + C::B_BYTES, d_last);
+          d_left = KV ? nt0 : nt1;
+          if (!KV) d_last = last1;
+        }
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + st * 2 * C::B_BYTES + C::B_BYTES, &bar->dp_full);
-        if (!KV) commit(&bar->b2_empty[st]);
-        if (!C::ATM && i + 1 == n) commit(&bar->a_empty[ab]);
+        issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + d_st.i * 2 * C::B_BYTES + C::B_BYTES,
+                     &bar->dp_full);
+        if (!KV) commit(&bar->b2_empty[d_st.i]);
+        d_st.next();
         return true;
       };
-      if (!do_s(0) || !do_dp(0)) break;
+      if (!do_s() || !do_dp()) break;
       bool ok = true;
-      for (int i = 0; i < n && ok; ++i, ph ^= 1u) {
-        const int st = (fill + i) % STAGES;
-        const uint32_t b1 = sB0 + st * 2 * C::B_BYTES, b2 = b1 + C::B_BYTES;
-        // S(i+1) as soon as its columns are free: S(i) is in registers, and
-        // (KV, P over S) P(i) is consumed, the MMAs running in order.  One
-        // stage only: its tile B1 takes the place of the one dS(i) still needs.
+      for (int left = n; left > 0; --left, ph ^= 1u) {
+        const bool more = left > 1, first = left == n;
+        const uint32_t b1 = sB0 + c_st.i * 2 * C::B_BYTES + dh_off, b2 = b1 + C::B_BYTES;
+        if (!C::ATM && !more) commit(&bar->a_empty[ab]);  // every S and dP of the item is issued
+        // The next S as soon as its columns are free: this S is in registers,
+        // and (KV, P over S) P is consumed, the MMAs running in order.  One
+        // stage only: its tile B1 takes the place of the one dS still needs.
         constexpr bool kEarlyS = C::SEP_P || !KV;
         if (kEarlyS && STAGES > 1) {
-          if (!wait(&bar->s_free, ph)) { ok = false; break; }
-          if (i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+          if (!wait(&bar->s_free, ph) || (more && !do_s())) { ok = false; break; }
         }
-        if constexpr (KV) {
-          if (!wait(&bar->p_full, ph)) { ok = false; break; }
-        }
-        if (i == 0) {
+        if (KV && !wait(&bar->p_full, ph)) { ok = false; break; }
+        if (first) {
           if (!wait(&bar->acc_empty, acc_ph)) { ok = false; break; }
           acc_ph ^= 1u;
         }
         if constexpr (KV) {
           tc_fence_after();
-          issue_acc(tmem_base + C::TM_ACC1, tmem_base + C::TM_P, C::SEP_P ? C::NC / 2 : C::NC, b2 + dh_off, i > 0,
-                    &bar->b2_empty[st]);
+          issue_acc(tmem_base + C::TM_ACC1, tmem_base + C::TM_P, C::SEP_P ? C::NC / 2 : C::NC, b2, !first,
+                    &bar->b2_empty[c_st.i]);
           if (C::SEP_P) commit(&bar->p_free);
         }
-        if (!kEarlyS && STAGES > 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
+        if (!kEarlyS && STAGES > 1 && more && !do_s()) { ok = false; break; }
         if (!wait(&bar->ds_full, ph)) { ok = false; break; }
         tc_fence_after();
-        issue_acc(tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1 + dh_off, i > 0, &bar->b1_empty[st]);
-        if (i + 1 == n) commit(&bar->acc_full);
-        if (STAGES == 1 && i + 1 < n && !do_s(i + 1)) { ok = false; break; }
-        if (i + 1 < n && !do_dp(i + 1)) { ok = false; break; }
+        issue_acc(tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1, !first, &bar->b1_empty[c_st.i]);
+        c_st.next();
+        if (more) {
+          if ((STAGES == 1 && !do_s()) || !do_dp()) { ok = false; break; }
+        } else {
+          commit(&bar->acc_full);
+        }
       }
       if (!ok) break;
-      fill += n;
     }
   } else {
     // ------------------------------------------------------------ element-wise warps + epilogue
