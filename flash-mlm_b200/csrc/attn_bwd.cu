@@ -168,7 +168,16 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.dkc = a->dk_context;
   p.dvc = a->dv_context;
   p.scale = a->scale;
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  // The exponent's scale, kept away from 0: the KV pass divides lse by it.  At
+  // 2^-24 scores of any size that float16 or bfloat16 attention meets (below a
+  // thousand) move the exponent by less than 2^-14.
+  const float sl2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = std::fabs(sl2) < 0x1p-24f ? (sl2 < 0.f ? -0x1p-24f : 0x1p-24f) : sl2;
+  // A power of two near 1 / scale_log2 (float16 holds 2^-14 .. 2^15), so that
+  // what the 16-bit columns hold is of lse's own magnitude.
+  const int e = std::min(15, std::max(-14, -std::ilogb(p.scale_log2)));
+  p.ext_unit = std::ldexp(1.f, e);
+  p.ext_mul = 1.f / (p.scale_log2 * p.ext_unit);
   p.err = a->error_word;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

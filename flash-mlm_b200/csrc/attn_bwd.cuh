@@ -16,7 +16,13 @@
 //   acc2 += dS B1,  KV: acc1 += P B2      (P, dS: 16-bit, A operand from TMEM)
 // In the KV pass S and dP are the transposed scores, so P^T and dS^T leave the
 // registers in the layout in which the tensor cores read A from TMEM, as in
-// the Q pass; P and dS never touch shared memory.
+// the Q pass; P and dS never touch shared memory.  lse and delta then belong
+// to columns: every thread would have to read all of them from shared memory,
+// 128 KB per tile through a 128-byte-a-cycle port (measured: 1800 + 1800 cycles
+// a tile for P and dS against 1000 + 650 in the Q pass).  Instead one more K
+// step of the score MMAs adds them: B gets 16 more columns that hold -lse (in
+// units of the scores) and -delta as sums of three 16-bit numbers, A the
+// matching constants, so S and dP arrive with them subtracted.
 //
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
@@ -40,10 +46,12 @@ struct BwdParams {
   int num_items;
   const int* cu_q;
   const int* cu_c;
-  const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta * 2^-kPExp}
+  const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta}
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
-  float scale, scale_log2;
+  float scale, scale_log2;  // scale_log2: of the scores in the exponent (never 0: see the host code)
+  float ext_unit;           // KV: A's constant (a power of two) for the lse columns
+  float ext_mul;            // KV: 1 / (scale_log2 * ext_unit)
   int* err;
   unsigned long long timeout_ns;
 };
@@ -68,7 +76,6 @@ struct BwdCfg {
   // operands in shared memory an MMA of 128 x 128 x 16 reads 8 KB in 64 cycles,
   // all that shared memory delivers, and every barrier and load waits behind it.
   static constexpr bool ATM = KV ? D <= 64 : D <= 128;
-  static constexpr int ABUF = D <= 64 ? 2 : 1;
   // P in columns of its own (KV): the next S need not wait until P is consumed.
   static constexpr bool SEP_P = KV && D <= 64;
   static constexpr int EW_GROUPS = 4;
@@ -83,11 +90,13 @@ struct BwdCfg {
   static constexpr int TMEM_USED = TM_A2 + (ATM ? D / 2 : 0);
   static_assert(TMEM_USED <= 512, "TMEM budget");
   static constexpr int TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
-  static constexpr int STAT_BYTES = KV ? STAGES * BN * 8 : 0;
-  static constexpr int SMEM_TILES = 2 * ABUF * A_BYTES + 2 * STAGES * B_BYTES;
+  // KV: the extra K step, 32-byte rows: A's constants, and per stage B1's and B2's columns
+  static constexpr int AX_BYTES = KV ? BM * 32 : 0;
+  static constexpr int BX_BYTES = KV ? BN * 32 : 0;
+  static constexpr int SMEM_TILES = 2 * A_BYTES + 2 * STAGES * B_BYTES + AX_BYTES + 2 * STAGES * BX_BYTES;
   static constexpr int RING = 4;
   static constexpr int ITEM_BYTES = 96;
-  static constexpr int SMEM_BYTES = SMEM_TILES + STAT_BYTES + 512 + RING * ITEM_BYTES + 1024;
+  static constexpr int SMEM_BYTES = SMEM_TILES + 512 + RING * ITEM_BYTES + 1024;
 };
 
 // A work item: the stationary tile, the rows it writes and up to two ranges of
@@ -198,7 +207,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
 }
 
 struct __align__(8) BwdBarriers {
-  uint64_t a_full[2], a_empty[2];
+  uint64_t a_full, a_empty;
   uint64_t b1_full[4], b2_full[4], b1_empty[4], b2_empty[4];
   uint64_t a_tm;              // element-wise -> MMA: the stationary tiles are in TMEM
   uint64_t s_full, dp_full;   // MMA -> element-wise: S / dP complete
@@ -262,6 +271,26 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// 16-byte half h of row r of a tile of 32-byte rows in the 32-byte swizzle.
+__device__ __forceinline__ uint8_t* ext_row(uint8_t* tile, int r, int h) {
+  return tile + r * 32 + ((h ^ ((r >> 2) & 1)) << 4);
+}
+
+// v as the sum of three 16-bit numbers (to 2^-27 of it in bfloat16, 2^-33 in
+// float16), float16's saturated.
+template <bool BF16>
+__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
+  if constexpr (BF16) {
+    a = __bfloat162float(__float2bfloat16_rn(v));
+    b = __bfloat162float(__float2bfloat16_rn(v - a));
+  } else {
+    a = __half2float(__float2half_rn(fminf(fmaxf(v, -65504.f), 65504.f)));
+    b = __half2float(__float2half_rn(fminf(fmaxf(v - a, -65504.f), 65504.f)));
+  }
+  c = v - a - b;
+  if constexpr (!BF16) c = fminf(fmaxf(c, -65504.f), 65504.f);
+}
+
 template <int D, bool KV, bool BF16>
 __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -273,10 +302,11 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   constexpr int BN = C::BN, SWB = C::SWB, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;                            // [ABUF][A1, A2]
-  uint8_t* sB = sA + 2 * C::ABUF * C::A_BYTES;   // [STAGES][B1, B2]
-  float* sStat = reinterpret_cast<float*>(sB + 2 * STAGES * C::B_BYTES);  // KV: [STAGES][2][BN]
-  BwdBarriers* bar = reinterpret_cast<BwdBarriers*>(reinterpret_cast<uint8_t*>(sStat) + C::STAT_BYTES);
+  uint8_t* sA = smem;                        // [A1, A2]
+  uint8_t* sB = sA + 2 * C::A_BYTES;         // [STAGES][B1, B2]
+  uint8_t* sAx = sB + 2 * STAGES * C::B_BYTES;  // KV: A's constants of the extra K step
+  uint8_t* sBx = sAx + C::AX_BYTES;             // KV: [STAGES][B1's, B2's extra columns]
+  BwdBarriers* bar = reinterpret_cast<BwdBarriers*>(smem + C::SMEM_TILES);
   BwdItem* ring_items = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(bar) + 512);
   volatile int* abort_flag = &bar->abort_flag;
 
@@ -284,12 +314,10 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->a_full[i], 1);
-      mbar_init(&bar->a_empty[i], C::ATM ? C::EW_WARPS : 1);
-    }
+    mbar_init(&bar->a_full, 1);
+    mbar_init(&bar->a_empty, C::ATM ? C::EW_WARPS : 1);
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&bar->b1_full[i], KV ? 2 : 1);  // KV: the tile, and its rows' stats
+      mbar_init(&bar->b1_full[i], KV ? 2 : 1);  // KV: the tile, and its rows' extra columns
       mbar_init(&bar->b2_full[i], 1);
       mbar_init(&bar->b1_empty[i], 1);
       mbar_init(&bar->b2_empty[i], 1);
@@ -311,6 +339,18 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   if (warp == C::MMA_WARP) {
     tmem_alloc(&bar->tmem_base, C::TMEM_COLS);
     tmem_relinquish();
+  }
+  if constexpr (KV) {
+    // Rows of 32 bytes in the 32-byte swizzle.  A's: the unit of the lse
+    // columns three times, 1 three times, zeros; B's second halves: zeros.
+    for (int r = threadIdx.x; r < C::BM; r += C::THREADS) {
+      const uint32_t u = pack2<BF16>(p.ext_unit, p.ext_unit), um = pack2<BF16>(p.ext_unit, 1.f), o = pack2<BF16>(1.f, 1.f);
+      *reinterpret_cast<uint4*>(ext_row(sAx, r, 0)) = make_uint4(u, um, o, 0);
+      *reinterpret_cast<uint4*>(ext_row(sAx, r, 1)) = make_uint4(0, 0, 0, 0);
+    }
+    for (int r = threadIdx.x; r < 2 * STAGES * BN; r += C::THREADS)
+      *reinterpret_cast<uint4*>(ext_row(sBx + (r / BN) * C::BX_BYTES, r % BN, 1)) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
   }
   if (warp == C::TMA_WARP && lane == 0) {
     tma_prefetch_desc(&tm_q);
@@ -378,15 +418,13 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       if (w >= num_items) break;
       const int n = it.heads * it.nt0 + it.nt1;
       if (n > 0) {
-        const int ab = aload % C::ABUF;
-        if (!wait(&bar->a_empty[ab], ((aload / C::ABUF) & 1u) ^ 1u)) break;
+        if (!wait(&bar->a_empty, (aload & 1u) ^ 1u)) break;
         if (lane == 0) {
           const CUtensorMap* m1 = KV ? (it.a_map ? &tm_kc : &tm_k) : &tm_q;
           const CUtensorMap* m2 = KV ? (it.a_map ? &tm_vc : &tm_v) : &tm_do;
-          uint8_t* dst = sA + ab * 2 * C::A_BYTES;
-          mbar_arrive_expect_tx(&bar->a_full[ab], 2 * C::A_BYTES);
-          load_tile(dst, m1, &bar->a_full[ab], C::BM, it.a_row, it.a_h, it.a_b);
-          load_tile(dst + C::A_BYTES, m2, &bar->a_full[ab], C::BM, it.a_row, it.a_h, it.a_b);
+          mbar_arrive_expect_tx(&bar->a_full, 2 * C::A_BYTES);
+          load_tile(sA, m1, &bar->a_full, C::BM, it.a_row, it.a_h, it.a_b);
+          load_tile(sA + C::A_BYTES, m2, &bar->a_full, C::BM, it.a_row, it.a_h, it.a_b);
         }
         __syncwarp();
         ++aload;
@@ -413,15 +451,21 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           }
           __syncwarp();
           if constexpr (KV) {
-            // The streamed rows' statistics; rows past the range get P = 0.
+            // The streamed rows' extra columns; rows past the range (their
+            // tile rows are cleared: S = dP = 0) get P = 2^-400 = 0.
             const float2* src = p.stats + it.stat0 + (long long)g * it.stat_h;
-            float* ss = sStat + st * 2 * BN;
+            uint8_t* x1 = sBx + st * 2 * C::BX_BYTES;
 #pragma unroll
             for (int c = lane; c < BN; c += 32) {
-              const float2 x = row + c < end ? __ldg(src + row + c) : make_float2(-INFINITY, 0.f);
-              ss[c] = x.x;
-              ss[BN + c] = x.y;
+              const float2 x = row + c < end ? __ldg(src + row + c) : make_float2(-400.f, 0.f);
+              float u, v, w;
+              split3<BF16>(x.x * p.ext_mul, u, v, w);
+              *reinterpret_cast<uint4*>(ext_row(x1, c, 0)) = make_uint4(pack2<BF16>(u, v), pack2<BF16>(w, 0.f), 0, 0);
+              split3<BF16>(x.y, u, v, w);
+              *reinterpret_cast<uint4*>(ext_row(x1 + C::BX_BYTES, c, 0)) =
+                  make_uint4(0, pack2<BF16>(0.f, u), pack2<BF16>(v, w), 0);
             }
+            fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->b1_full[st]);
           }
@@ -437,14 +481,17 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     constexpr uint32_t idesc_s = make_idesc_f16(fmt, 0, 0, C::BM, BN);
     constexpr uint32_t idesc_acc = make_idesc_f16(fmt, 0, 1, C::BM, C::DV);
     constexpr uint32_t layout = swizzle_code(SWB);
-    const uint32_t sA0 = smem_u32(sA), sB0 = smem_u32(sB);
+    const uint32_t a1 = smem_u32(sA), a2 = a1 + C::A_BYTES, sB0 = smem_u32(sB);
+    const uint32_t ax = (smem_u32(sAx) >> 4) | (1u << 16), bx0 = (smem_u32(sBx) >> 4) | (1u << 16);
+    constexpr uint32_t hi_x = (256u >> 4) | (1u << 14) | (swizzle_code(32) << 29);  // 32-byte rows
     const bool leader = elect_one();
     // high descriptor word: 8-row stride, descriptor version 1, swizzle
     constexpr uint32_t hi = (8 * SWB >> 4) | (1u << 14) | (layout << 29);
     constexpr uint32_t lbo_k = 1u << 16;                // K-major: unused
     constexpr uint32_t lbo_mn = (BN * SWB >> 4) << 16;  // MN-major: slab stride
-    // scores: D[128, BN] = A[128, D] B[BN, D]^T (A in TMEM or shared memory), then commit to `done`
-    auto issue_scores = [&](uint32_t d, uint32_t a_tm, uint32_t a_base, uint32_t b_base, uint64_t* done) {
+    // scores: D[128, BN] = A[128, D] B[BN, D]^T (A in TMEM or shared memory;
+    // KV: and the extra columns bx), then commit to `done`
+    auto issue_scores = [&](uint32_t d, uint32_t a_tm, uint32_t a_base, uint32_t b_base, uint32_t bx, uint64_t* done) {
       if (leader) {
         const uint32_t a = (a_base >> 4) | lbo_k, b = (b_base >> 4) | lbo_k;
 #pragma unroll
@@ -454,6 +501,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           if constexpr (C::ATM) mma_ts(d, a_tm + kk * 8, bk, hi, idesc_s, kk > 0 ? 1u : 0u);
           else mma_ss(d, a + ((slab * (C::BM * SWB) + inrow) >> 4), bk, hi, idesc_s, kk > 0 ? 1u : 0u);
         }
+        if constexpr (KV) mma_ss(d, ax, bx, hi_x, idesc_s, 1u);
         umma_commit(done);
       }
     };
@@ -508,10 +556,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const uint32_t dh_off = (slot->dh * C::DV / C::SLAB_COLS) * (BN * SWB);
       release_item(ring);
       if (n == 0) continue;
-      const int ab = aload % C::ABUF;
-      if (!wait(C::ATM ? &bar->a_tm : &bar->a_full[ab], C::ATM ? (aload & 1u) : (aload / C::ABUF) & 1u)) break;
+      if (!wait(C::ATM ? &bar->a_tm : &bar->a_full, aload & 1u)) break;
       ++aload;
-      const uint32_t a1 = sA0 + ab * 2 * C::A_BYTES, a2 = a1 + C::A_BYTES;
       // Tiles left in the range that S / dP walk, and that range's last tile.
       int s_left = nt0 > 0 ? nt0 : nt1, d_left = s_left;
       int s_last = nt0 > 0 ? last0 : last1, d_last = s_last;
@@ -523,7 +569,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           if (!KV) s_last = last1;
         }
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + s_st.i * 2 * C::B_BYTES, &bar->s_full);
+        issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + s_st.i * 2 * C::B_BYTES,
+                     bx0 + s_st.i * (2 * C::BX_BYTES >> 4), &bar->s_full);
         s_st.next();
         return true;
       };
@@ -536,7 +583,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         }
         tc_fence_after();
         issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + d_st.i * 2 * C::B_BYTES + C::B_BYTES,
-                     &bar->dp_full);
+                     bx0 + ((d_st.i * 2 + 1) * C::BX_BYTES >> 4), &bar->dp_full);
         if (!KV) commit(&bar->b2_empty[d_st.i]);
         d_st.next();
         return true;
@@ -546,7 +593,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       for (int left = n; left > 0; --left, ph ^= 1u) {
         const bool more = left > 1, first = left == n;
         const uint32_t b1 = sB0 + c_st.i * 2 * C::B_BYTES + dh_off, b2 = b1 + C::B_BYTES;
-        if (!C::ATM && !more) commit(&bar->a_empty[ab]);  // every S and dP of the item is issued
+        if (!C::ATM && !more) commit(&bar->a_empty);  // every S and dP of the item is issued
         // The next S as soon as its columns are free: this S is in registers,
         // and (KV, P over S) P is consumed, the MMAs running in order.  One
         // stage only: its tile B1 takes the place of the one dS still needs.
@@ -589,7 +636,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
     const float sl2 = p.scale_log2;
     constexpr float kInv = BwdScale<BF16>::kInv;
-    uint32_t fill = 0, ph = 0, acc_ph = 0, aload = 0;
+    uint32_t ph = 0, acc_ph = 0, aload = 0;
     auto arrive = [&](uint64_t* b) {
       tc_fence_before();
       __syncwarp();
@@ -605,13 +652,12 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     // Stationary tiles, shared memory -> TMEM: half the warps copy A1, half A2,
     // (D > 16) each warp half of its rows' columns.
     auto copy_a = [&]() -> bool {
-      const int ab = aload % C::ABUF;
-      if (!wait(&bar->a_full[ab], (aload / C::ABUF) & 1u)) return false;
+      if (!wait(&bar->a_full, aload & 1u)) return false;
       ++aload;
       constexpr int W = D > 16 ? D / 4 : 8;  // 32-bit words per thread
       const int half = D > 16 ? g & 1 : 0;
       if (D > 16 || (g & 1) == 0) {
-        const uint8_t* tile = sA + ab * 2 * C::A_BYTES + (g >> 1) * C::A_BYTES;
+        const uint8_t* tile = sA + (g >> 1) * C::A_BYTES;
         uint32_t v[W];
 #pragma unroll
         for (int c = 0; c < W / 4; ++c) {
@@ -625,7 +671,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         else tmem_st_x8(dst, v);
       }
       arrive(&bar->a_tm);
-      if (lane == 0) mbar_arrive(&bar->a_empty[ab]);
+      if (lane == 0) mbar_arrive(&bar->a_empty);
       return true;
     };
     const BwdItem* it = take_item(0);
@@ -634,10 +680,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int nt0 = it->nt0, n = it->heads * nt0 + it->nt1;
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
-      for (int i = 0; i < n; ++i, ++fill, ph ^= 1u) {
-        const int stg = fill % STAGES;
-        const float* ss = sStat + stg * 2 * BN + g * NC;
-        if (KV && !wait(&bar->b1_full[stg], (fill / STAGES) & 1u)) break;
+      for (int i = 0; i < n; ++i, ph ^= 1u) {
         if (!wait(&bar->s_full, ph)) break;
         tc_fence_after();
         uint32_t x[NC];
@@ -646,13 +689,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         if (C::SEP_P || !KV) arrive(&bar->s_free);
         if constexpr (KV) {
 #pragma unroll
-          for (int c = 0; c < NC; c += 4) {
-            const float4 nl = *reinterpret_cast<const float4*>(ss + c);
-            pr[c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, nl.x));
-            pr[c + 1] = ex2_approx(fmaf(__uint_as_float(x[c + 1]), sl2, nl.y));
-            pr[c + 2] = ex2_approx(fmaf(__uint_as_float(x[c + 2]), sl2, nl.z));
-            pr[c + 3] = ex2_approx(fmaf(__uint_as_float(x[c + 3]), sl2, nl.w));
-          }
+          for (int c = 0; c < NC; ++c) pr[c] = ex2_approx(__uint_as_float(x[c]) * sl2);
           uint32_t pk[NC / 2];
 #pragma unroll
           for (int c = 0; c < NC / 2; ++c) pk[c] = pack2<BF16>(pr[2 * c], pr[2 * c + 1]);
@@ -677,14 +714,17 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         ld(tDP, x);
         uint32_t pk[NC / 2];
 #pragma unroll
-        for (int c = 0; c < NC; c += 4) {
-          float4 nd;
-          if constexpr (KV) nd = *reinterpret_cast<const float4*>(ss + BN + c);
-          else nd = make_float4(rs.y, rs.y, rs.y, rs.y);
-          pk[c / 2] = pack2<BF16>(pr[c] * fmaf(__uint_as_float(x[c]), kInv, nd.x),
-                                  pr[c + 1] * fmaf(__uint_as_float(x[c + 1]), kInv, nd.y));
-          pk[c / 2 + 1] = pack2<BF16>(pr[c + 2] * fmaf(__uint_as_float(x[c + 2]), kInv, nd.z),
-                                      pr[c + 3] * fmaf(__uint_as_float(x[c + 3]), kInv, nd.w));
+        for (int c = 0; c < NC; c += 2) {
+          float d0 = __uint_as_float(x[c]), d1 = __uint_as_float(x[c + 1]);
+          if constexpr (!KV) {
+            d0 += rs.y;
+            d1 += rs.y;
+          }
+          if constexpr (!BF16) {
+            d0 *= kInv;
+            d1 *= kInv;
+          }
+          pk[c / 2] = pack2<BF16>(pr[c] * d0, pr[c + 1] * d1);
         }
         st16(tDP, pk);
         arrive(&bar->ds_full);
@@ -751,7 +791,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   }
 }
 
-// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O) * 2^-kPExp}; also
+// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}; also
 // zeroes the item counters of the two passes that follow.  Reads O and dO
 // once (bound by HBM).  delta uses the 16-bit O that the forward pass returned:
 // its rounding (half a step per element) enters dS as |dO| * 2^-9 noise, below
@@ -785,7 +825,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const uint4* __rest
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (r < rows && threadIdx.x % LANES == 0)
-    stats[r] = make_float2(fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp), -s * BwdScale<BF16>::kInv);
+    stats[r] = make_float2(fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp), -s);
 }
 
 }  // namespace fmlm
