@@ -252,6 +252,38 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tm, uint32_t b_lo,
       : "memory");
 }
 
+// Two float32 operations in one instruction (sm_100): the element-wise warps
+// are bound by issue slots and the exponentials' unit, not by arithmetic.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2u(uint32_t a, uint32_t b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ void unf2(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
 // 16-byte vector c of row r of a K-major tile as TMA's swizzle laid it out.
 template <int SWB>
 __device__ __forceinline__ uint4 ld_swizzled(const uint8_t* tile, int rows, int r, int c) {
@@ -269,6 +301,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&v);
   }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(F2 v) {
+  float a, b;
+  unf2(v, a, b);
+  return pack2<BF16>(a, b);
 }
 
 // 16-byte half h of row r of a tile of 32-byte rows in the 32-byte swizzle.
@@ -634,8 +673,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint32_t tS = tmem_base + lane_off + C::TM_S + g * NC;
     const uint32_t tDP = tmem_base + lane_off + C::TM_DP + g * NC;
     const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
-    const float sl2 = p.scale_log2;
     constexpr float kInv = BwdScale<BF16>::kInv;
+    const F2 sl2_2 = f2(p.scale_log2, p.scale_log2), kinv_2 = f2(kInv, kInv);
     uint32_t ph = 0, acc_ph = 0, aload = 0;
     auto arrive = [&](uint64_t* b) {
       tc_fence_before();
@@ -680,19 +719,25 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int nt0 = it->nt0, n = it->heads * nt0 + it->nt1;
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
+      const F2 nl_2 = f2(rs.x, rs.x), nd_2 = f2(rs.y * kInv, rs.y * kInv);
       for (int i = 0; i < n; ++i, ph ^= 1u) {
         if (!wait(&bar->s_full, ph)) break;
         tc_fence_after();
         uint32_t x[NC];
-        float pr[NC];
+        F2 pr[NC / 2];
         ld(tS, x);
         if (C::SEP_P || !KV) arrive(&bar->s_free);
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) {
+          const F2 xs = f2u(x[2 * c], x[2 * c + 1]);
+          float a, b;
+          unf2(KV ? mul2(xs, sl2_2) : fma2(xs, sl2_2, nl_2), a, b);
+          pr[c] = f2(ex2_approx(a), ex2_approx(b));
+        }
+        uint32_t pk[NC / 2];
         if constexpr (KV) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c) pr[c] = ex2_approx(__uint_as_float(x[c]) * sl2);
-          uint32_t pk[NC / 2];
-#pragma unroll
-          for (int c = 0; c < NC / 2; ++c) pk[c] = pack2<BF16>(pr[2 * c], pr[2 * c + 1]);
+          for (int c = 0; c < NC / 2; ++c) pk[c] = pack2<BF16>(pr[c]);
           if (C::SEP_P) {
             if (!wait(&bar->p_free, ph ^ 1u)) break;
             tc_fence_after();
@@ -700,31 +745,25 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           st16(tP, pk);
           arrive(&bar->p_full);
         } else {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) pr[c] = ex2_approx(fmaf(__uint_as_float(x[c]), sl2, rs.x));
           const int valid = (i >= nt0 ? it->end1 - (it->row1 + (i - nt0) * BN) : it->end0 - (it->row0 + i * BN)) - g * NC;
           if (valid < NC) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-              if (c >= valid) pr[c] = 0.f;
+            for (int c = 0; c < NC / 2; ++c) {
+              float a, b;
+              unf2(pr[c], a, b);
+              pr[c] = f2(2 * c < valid ? a : 0.f, 2 * c + 1 < valid ? b : 0.f);
+            }
           }
         }
         if (!wait(&bar->dp_full, ph)) break;
         tc_fence_after();
         ld(tDP, x);
-        uint32_t pk[NC / 2];
 #pragma unroll
-        for (int c = 0; c < NC; c += 2) {
-          float d0 = __uint_as_float(x[c]), d1 = __uint_as_float(x[c + 1]);
-          if constexpr (!KV) {
-            d0 += rs.y;
-            d1 += rs.y;
-          }
-          if constexpr (!BF16) {
-            d0 *= kInv;
-            d1 *= kInv;
-          }
-          pk[c / 2] = pack2<BF16>(pr[c] * d0, pr[c + 1] * d1);
+        for (int c = 0; c < NC / 2; ++c) {
+          F2 d = f2u(x[2 * c], x[2 * c + 1]);
+          if constexpr (!KV) d = fma2(d, kinv_2, nd_2);
+          else if constexpr (!BF16) d = mul2(d, kinv_2);
+          pk[c] = pack2<BF16>(mul2(pr[c], d));
         }
         st16(tDP, pk);
         arrive(&bar->ds_full);
