@@ -248,6 +248,18 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(fn, device: torch.device, what: str, *args) -> None:
+    """Call a C entry point whose last argument is the stream: `device`'s current one, with `device` current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc, what)
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.float16:
         return FMLM_DTYPE_F16

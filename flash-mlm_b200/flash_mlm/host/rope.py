@@ -15,7 +15,7 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
-from flash_mlm.host.host_utils import require_cuda_tensors, validate_head_dim_supported
+from flash_mlm.host.host_utils import validate_head_dim_supported
 
 _PAIRS = {"half": _lib.FMLM_PAIRS_HALF, "interleaved": _lib.FMLM_PAIRS_INTERLEAVED}
 
@@ -49,25 +49,32 @@ class RotaryTable:
 
 def _rows_ready(x: torch.Tensor) -> torch.Tensor:
     """x itself if its rows can be read in 16-byte vectors where they lie, else a contiguous copy."""
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in x.stride()[:-1])
+    *outer, last = x.stride()
+    ok = last == 1 and x.data_ptr() % 16 == 0
+    for stride in outer:
+        ok = ok and stride % 8 == 0
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
 def _view(x: torch.Tensor) -> _lib.View4:
     if x.ndim == 4:
-        return _lib.view_bhnd(x)
-    return _lib.view4(x, rows=x.shape[1], heads=x.shape[0], batch=1, row_stride=x.stride(1), head_stride=x.stride(0))
+        b, h, n, _ = x.shape
+        sb, sh, sn, _ = x.stride()
+        return _lib.View4(x.data_ptr(), n, h, b, sn, sh, sb)
+    h, t, _ = x.shape
+    sh, st, _ = x.stride()
+    return _lib.View4(x.data_ptr(), t, h, 1, st, sh, 0)
 
 
 def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
     if q.ndim not in (3, 4) or k.ndim != q.ndim:
         raise ValueError("q/k must be rank-4 tensors [B, H, N, D] or packed rank-3 tensors [H, T, D]")
-    h = q.ndim - 3
-    if q.shape[:h] != k.shape[:h] or q.shape[h + 1:] != k.shape[h + 1:]:
+    qs, ks = q.shape, k.shape
+    if qs[-2:] != ks[-2:] or (q.ndim == 4 and qs[0] != ks[0]):
         raise ValueError("q and k may differ in their number of heads only")
-    if q.shape[h] < 1 or k.shape[h] < 1:
+    if qs[-3] < 1 or ks[-3] < 1:
         raise ValueError("q and k must have at least one head")
-    d = q.shape[-1]
+    d = qs[-1]
     validate_head_dim_supported(d)
     _lib.dtype_code(q.dtype)
     if k.dtype != q.dtype:
@@ -75,22 +82,23 @@ def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, position
     if q.ndim == 3:
         if q_meta is None:
             raise ValueError("packed q/k need q_meta")
-        if q_meta.total_tokens != q.shape[1] or q_meta.token_indices.numel() != q.shape[1]:
+        if q_meta.total_tokens != qs[1] or q_meta.token_indices.numel() != qs[1]:
             raise ValueError("packed token count mismatch with PackMetadata")
-    elif q_meta is not None and (q_meta.B != q.shape[0] or q_meta.N != q.shape[2]):
+    elif q_meta is not None and (q_meta.B != qs[0] or q_meta.N != qs[2]):
         raise ValueError("q_meta shape metadata does not match q/k padded shape")
     if rotary is None and not normalize:
         raise ValueError("nothing to do: give rotary, or normalize=True")
     if rotary is not None and rotary.rotary_dim > d:
         raise ValueError("rotary_dim must be at most head_dim")
-    tensors = [q, k] + ([rotary.table] if rotary is not None else [])
+    tensors = [q, k] if rotary is None else [q, k, rotary.table]
     weights = [w for w in (q_weight, k_weight) if w is not None]
     if weights and not normalize:
         raise ValueError("weights need normalize=True")
-    if any(tuple(w.shape) != (d,) for w in weights):
-        raise ValueError("q_weight and k_weight must be [head_dim]")
-    if any(w.dtype not in (torch.float32, q.dtype) or w.dtype != weights[0].dtype for w in weights):
-        raise ValueError("q_weight and k_weight must both be float32, or both of q's dtype")
+    for w in weights:
+        if tuple(w.shape) != (d,):
+            raise ValueError("q_weight and k_weight must be [head_dim]")
+        if (w.dtype != torch.float32 and w.dtype != q.dtype) or w.dtype != weights[0].dtype:
+            raise ValueError("q_weight and k_weight must both be float32, or both of q's dtype")
     if normalize and not eps >= 0.0:
         raise ValueError("eps must be >= 0")
     tensors += weights
@@ -112,9 +120,12 @@ def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, position
         tensors += [q_meta.lengths, q_meta.token_indices]
         if q_meta.lengths.dtype != torch.int32 or q_meta.token_indices.dtype != torch.int64:
             raise ValueError("q_meta must hold int32 lengths and int64 token_indices")
-    require_cuda_tensors(*tensors)
-    if any(x.device != q.device for x in tensors):
-        raise ValueError("all tensors must be on q's device")
+    if not q.is_cuda:
+        raise ValueError("All tensors must be CUDA tensors")
+    device = q.device
+    for x in tensors:
+        if x.device != device:
+            raise ValueError("all tensors must be on q's device")
 
 
 def _args(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
@@ -131,7 +142,8 @@ def _args(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, p
     def ptr(x, dtype=None):
         if x is None:
             return None
-        x = x.detach().contiguous()
+        if not x.is_contiguous():
+            x = x.detach().contiguous()
         keep.append(x)
         return x.data_ptr()
 
@@ -160,8 +172,7 @@ def _forward(q, k, *call):
     if q.numel() and k.numel():
         a, keep = _args(_rows_ready(q), _rows_ready(k), *call)
         a.q_out, a.k_out = out_q.data_ptr(), out_k.data_ptr()
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().fmlm_qk_rope_fwd(ctypes.byref(a), _lib.stream_ptr(q.device)), "qk_norm_rope")
+        _lib.launch(_lib.lib().fmlm_qk_rope_fwd, q.device, "qk_norm_rope", ctypes.byref(a))
         del keep
     return out_q, out_k
 
@@ -174,32 +185,38 @@ class _QkNormRope(torch.autograd.Function):
         return _forward(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, positions, position_offsets = ctx.saved_tensors
-        rotary, normalize, eps, q_meta = ctx.call
-        dq, dk = _outputs(q, k)
-        dwq, dwk = (torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and need else None
-                    for w, need in ((q_weight, ctx.needs_input_grad[2]), (k_weight, ctx.needs_input_grad[3])))
-        if not (q.numel() and k.numel()):
-            for w in (dwq, dwk):
-                if w is not None:
-                    w.zero_()
-            return dq, dk, dwq, dwk, None, None, None, None, None, None
-        a, keep = _args(_rows_ready(q), _rows_ready(k), rotary, q_weight, k_weight, normalize, eps, q_meta, positions,
-                        position_offsets)
-        gq, gk = _rows_ready(gq), _rows_ready(gk)
-        a.gq, a.gk = _view(gq), _view(gk)
-        a.q_out, a.k_out = dq.data_ptr(), dk.data_ptr()
-        if dwq is not None or dwk is not None:
-            a.dq_weight, a.dk_weight = (None if w is None else w.data_ptr() for w in (dwq, dwk))
-            nbytes = _lib.lib().fmlm_qk_rope_bwd_workspace_bytes(q.shape[-1])
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        with torch.cuda.device(q.device):
-            _lib.check(_lib.lib().fmlm_qk_rope_bwd(ctypes.byref(a), _lib.stream_ptr(q.device)), "qk_norm_rope backward")
-        del keep
+        # (the wrapper marks the gradients as not differentiable again; without create_graph nothing could be)
+        return _rope_backward_once(ctx, gq, gk) if torch.is_grad_enabled() else _rope_backward(ctx, gq, gk)
+
+
+def _rope_backward(ctx, gq, gk):
+    q, k, q_weight, k_weight, positions, position_offsets = ctx.saved_tensors
+    rotary, normalize, eps, q_meta = ctx.call
+    dq, dk = _outputs(q, k)
+    dwq, dwk = (torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and need else None
+                for w, need in ((q_weight, ctx.needs_input_grad[2]), (k_weight, ctx.needs_input_grad[3])))
+    if not (q.numel() and k.numel()):
+        for w in (dwq, dwk):
+            if w is not None:
+                w.zero_()
         return dq, dk, dwq, dwk, None, None, None, None, None, None
+    a, keep = _args(_rows_ready(q), _rows_ready(k), rotary, q_weight, k_weight, normalize, eps, q_meta, positions,
+                    position_offsets)
+    gq, gk = _rows_ready(gq), _rows_ready(gk)
+    a.gq, a.gk = _view(gq), _view(gk)
+    a.q_out, a.k_out = dq.data_ptr(), dk.data_ptr()
+    if dwq is not None or dwk is not None:
+        a.dq_weight, a.dk_weight = (None if w is None else w.data_ptr() for w in (dwq, dwk))
+        nbytes = _lib.lib().fmlm_qk_rope_bwd_workspace_bytes(q.shape[-1])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.launch(_lib.lib().fmlm_qk_rope_bwd, q.device, "qk_norm_rope backward", ctypes.byref(a))
+    del keep
+    return dq, dk, dwq, dwk, None, None, None, None, None, None
+
+
+_rope_backward_once = torch.autograd.function.once_differentiable(_rope_backward)
 
 
 def qk_norm_rope(

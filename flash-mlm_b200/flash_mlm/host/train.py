@@ -30,14 +30,16 @@ import torch
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
-from flash_mlm.host.host_utils import pack_for_kernel, require_cuda_tensors, unpack_from_kernel, validate_head_dim_supported
+from flash_mlm.host.host_utils import pack_for_kernel, unpack_from_kernel, validate_head_dim_supported
 
 
 def _tma_ready(x: torch.Tensor) -> torch.Tensor:
     """x itself if TMA can address its rows (16-byte aligned, positive strides), else a contiguous copy."""
-    d = x.shape[-1]
-    ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and x.stride(-2) >= d and x.stride(-2) % 8 == 0
-    for size, stride in zip(x.shape[:-2], x.stride()[:-2]):
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
+    *outer, row, last = x.stride()
+    ok = last == 1 and x.data_ptr() % 16 == 0 and row >= x.shape[-1] and row % 8 == 0
+    for size, stride in zip(x.shape, outer):
         ok = ok and (size == 1 or (stride > 0 and stride % 8 == 0))
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
@@ -45,10 +47,12 @@ def _tma_ready(x: torch.Tensor) -> torch.Tensor:
 def _view(x: torch.Tensor) -> _lib.View4:
     """[B, H, N, D] or [H, T, D] as a [batch][heads][rows] view."""
     if x.ndim == 4:
-        return _lib.view_bhnd(x)
+        b, h, n, _ = x.shape
+        sb, sh, sn, _ = x.stride()
+        return _lib.View4(x.data_ptr(), n, h, b, sn, sh, sb)
     h, t, d = x.shape
-    return _lib.view4(x, rows=t, heads=h, batch=1, row_stride=x.stride(1), head_stride=x.stride(0),
-                      batch_stride=h * t * d)
+    sh, st, _ = x.stride()
+    return _lib.View4(x.data_ptr(), t, h, 1, st, sh, h * t * d)
 
 
 def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
@@ -57,13 +61,13 @@ def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
         raise ValueError("q/k/v must be rank-4 tensors [B, H, N, D] or packed rank-3 tensors [H, T, D]")
     if k.shape != v.shape:
         raise ValueError("k and v must have the same shape")
-    hdim = q.ndim - 3
-    if q.shape[:hdim] != k.shape[:hdim] or q.shape[hdim + 1:] != k.shape[hdim + 1:]:
+    qs, ks = q.shape, k.shape
+    if qs[-2:] != ks[-2:] or (q.ndim == 4 and qs[0] != ks[0]):
         raise ValueError("q and k may differ in their number of heads only")
-    h, hk = q.shape[hdim], k.shape[hdim]
+    h, hk = qs[-3], ks[-3]
     if hk < 1 or h < 1 or h % hk != 0:
         raise ValueError("the heads of q must be a multiple of the heads of k and v")
-    validate_head_dim_supported(q.shape[-1])
+    validate_head_dim_supported(qs[-1])
     _lib.dtype_code(q.dtype)
     packed = q.ndim == 3
     if packed:
@@ -73,29 +77,33 @@ def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
             raise ValueError("packed token count mismatch with PackMetadata")
     elif q_meta is not None and (q_meta.B != q.shape[0] or q_meta.N != q.shape[2]):
         raise ValueError("q_meta shape metadata does not match q/k/v padded shape")
-    given = [x is not None for x in (context_k, context_v, context_meta)]
-    if any(given) and not all(given):
+    context = context_k is not None
+    if (context_v is not None) != context or (context_meta is not None) != context:
         raise ValueError("context_k, context_v and context_meta must be provided together or all omitted")
-    if (all(given) or causal) and q_meta is None:
+    if (context or causal) and q_meta is None:
         raise ValueError("a context and causal_query_seq_attn need q_meta")
     tensors = [q, k, v]
-    if all(given):
-        d = q.shape[-1]
-        if context_k.shape != (hk, context_meta.total_tokens, d) or context_v.shape != context_k.shape:
+    if context:
+        if context_k.shape != (hk, context_meta.total_tokens, qs[-1]) or context_v.shape != context_k.shape:
             raise ValueError("context_k and context_v must be [heads of k, context_meta.total_tokens, D]")
         if context_meta.B not in (1, q_meta.B):
             raise ValueError("context_meta must describe one context, or one for every sequence")
         tensors += [context_k, context_v]
-    if any(x.dtype != q.dtype for x in tensors):
-        raise ValueError("q, k, v and the context must have the same dtype")
-    if any(x.device != q.device for x in tensors):
-        raise ValueError("q, k, v and the context must be on the same device")
-    metas = [m.cu_seqlens for m in (q_meta, context_meta) if m is not None]
-    require_cuda_tensors(*tensors, *metas)
-    if any(m.device != q.device for m in metas):
-        raise ValueError("q_meta and context_meta must be on q's device")
-    if any(m.dtype != torch.int32 or not m.is_contiguous() for m in metas):
-        raise ValueError("cu_seqlens must be contiguous int32")
+    dtype, device = q.dtype, q.device
+    for x in tensors:
+        if x.dtype != dtype:
+            raise ValueError("q, k, v and the context must have the same dtype")
+        if x.device != device:
+            raise ValueError("q, k, v and the context must be on the same device")
+    for m in (q_meta, context_meta):
+        if m is not None:
+            cu = m.cu_seqlens
+            if cu.device != device:
+                raise ValueError("q_meta and context_meta must be on q's device")
+            if cu.dtype != torch.int32 or not cu.is_contiguous() or cu.numel() != m.B + 1:
+                raise ValueError("cu_seqlens must be contiguous int32 of B + 1 elements")
+    if not q.is_cuda:
+        raise ValueError("All tensors must be CUDA tensors")
     if packed:
         return _lib.FMLM_BWD_PACKED
     return _lib.FMLM_BWD_DENSE if q_meta is None else _lib.FMLM_BWD_PADDED
@@ -135,6 +143,11 @@ def flash_attn_mlm_fwd(
     """
     layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     _require_packed(q, context_k, causal_query_seq_attn)
+    return _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+
+
+def _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta, causal):
+    """``flash_attn_mlm_fwd`` on checked arguments."""
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
     if _nothing_to_do(q, q_meta):
@@ -156,7 +169,7 @@ def flash_attn_mlm_fwd(
         packed = layout == _lib.FMLM_BWD_PACKED
         args = _lib.PackedArgs()
         args.dtype, args.head_dim, args.num_heads, args.batch = _lib.dtype_code(q.dtype), d, h, q_meta.B
-        args.causal_query_seq_attn = int(causal_query_seq_attn)
+        args.causal_query_seq_attn = int(causal)
         args.context_batch_size = 1
         args.scale = float(scale)
         args.q_layout = args.kv_layout = _lib.FMLM_LAYOUT_PACKED if packed else _lib.FMLM_LAYOUT_PADDED
@@ -174,8 +187,7 @@ def flash_attn_mlm_fwd(
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         args.workspace, args.workspace_bytes, args.error_word = ws.data_ptr(), nbytes, err.data_ptr()
         launch = L.fmlm_attn_packed_fwd_lse
-    with torch.cuda.device(q.device):
-        _lib.check(launch(ctypes.byref(args), hk, lse.data_ptr(), _lib.stream_ptr(q.device)), "flash_attn_mlm_fwd")
+    _lib.launch(launch, q.device, "flash_attn_mlm_fwd", ctypes.byref(args), hk, lse.data_ptr())
     return out, lse
 
 
@@ -210,6 +222,13 @@ def flash_attn_mlm_bwd(
             raise ValueError(f"{name} must have q's shape, dtype and device")
     if lse.shape != q.shape[:-1] or lse.dtype != torch.float32 or lse.device != q.device:
         raise ValueError("lse must be float32 of q's shape without the head dimension, on q's device")
+    return _backward(layout, dout, q, k, v, out, lse, scale, q_meta, context_k, context_v, context_meta,
+                     causal_query_seq_attn, need_dq, need_dkv)
+
+
+def _backward(layout, dout, q, k, v, out, lse, scale, q_meta, context_k, context_v, context_meta, causal, need_dq,
+              need_dkv):
+    """``flash_attn_mlm_bwd`` on checked arguments."""
     dev = q.device
 
     def like(x, wanted):
@@ -225,7 +244,7 @@ def flash_attn_mlm_bwd(
             if g is not None:
                 g.zero_()
         return grads
-    q, k, v, dout = (_tma_ready(x) for x in (q, k, v, dout))
+    q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
     dout, out, lse = _tma_ready(dout.contiguous()), _tma_ready(out.contiguous()), lse.contiguous()
     packed = layout == _lib.FMLM_BWD_PACKED
     L = _lib.lib()
@@ -234,7 +253,7 @@ def flash_attn_mlm_bwd(
     args.batch = q_meta.B if packed else q.shape[0]
     args.num_heads, args.kv_heads = q.shape[-3], k.shape[-3]
     args.seq_len = 0 if packed else q.shape[2]
-    args.causal_query_seq_attn = int(causal_query_seq_attn)
+    args.causal_query_seq_attn = int(causal)
     args.scale = float(scale)
     args.total_q_len = q.shape[1] if packed else 0
     args.q, args.k, args.v, args.dout = _view(q), _view(k), _view(v), _view(dout)
@@ -251,28 +270,34 @@ def flash_attn_mlm_bwd(
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
     args.error_word = _lib.error_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        _lib.check(L.fmlm_attn_bwd(ctypes.byref(args), _lib.stream_ptr(dev)), "flash_attn_mlm_bwd")
+    _lib.launch(L.fmlm_attn_bwd, dev, "flash_attn_mlm_bwd", ctypes.byref(args))
     return grads
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, context_k, context_v, scale, q_meta, context_meta, causal):
-        out, lse = flash_attn_mlm_fwd(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal)
+    def forward(ctx, q, k, v, context_k, context_v, layout, scale, q_meta, context_meta, causal):
+        out, lse = _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta, causal)
         ctx.save_for_backward(q, k, v, context_k, context_v, out, lse)
-        ctx.call = (scale, q_meta, context_meta, causal)
+        ctx.call = (layout, scale, q_meta, context_meta, causal)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, context_k, context_v, out, lse = ctx.saved_tensors
-        scale, q_meta, context_meta, causal = ctx.call
-        need = ctx.needs_input_grad
-        grads = flash_attn_mlm_bwd(dout, q, k, v, out, lse, scale, q_meta, context_k, context_v, context_meta, causal,
-                                   need_dq=need[0], need_dkv=any(need[1:5]))
-        return (*grads, None, None, None, None)
+        # (the wrapper marks the gradients as not differentiable again; without create_graph nothing could be)
+        return _attention_backward_once(ctx, dout) if torch.is_grad_enabled() else _attention_backward(ctx, dout)
+
+
+def _attention_backward(ctx, dout):
+    q, k, v, context_k, context_v, out, lse = ctx.saved_tensors
+    layout, scale, q_meta, context_meta, causal = ctx.call
+    need = ctx.needs_input_grad
+    grads = _backward(layout, dout, q, k, v, out, lse, scale, q_meta, context_k, context_v, context_meta, causal,
+                      need[0], any(need[1:5]))
+    return (*grads, None, None, None, None, None)
+
+
+_attention_backward_once = torch.autograd.function.once_differentiable(_attention_backward)
 
 
 class _Pack(torch.autograd.Function):
@@ -325,9 +350,10 @@ def flash_attn_mlm_train(
     To capture the backward pass into a CUDA graph, call ``flash_attn_mlm_fwd``
     and ``flash_attn_mlm_bwd``, which involve no autograd graph.
     """
-    _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     if q.ndim == 4 and (context_k is not None or causal_query_seq_attn):
         qp, kp, vp = (_Pack.apply(x, q_meta) for x in (q, k, v))
-        out = _Attention.apply(qp, kp, vp, context_k, context_v, scale, q_meta, context_meta, causal_query_seq_attn)
+        out = _Attention.apply(qp, kp, vp, context_k, context_v, _lib.FMLM_BWD_PACKED, scale, q_meta, context_meta,
+                               causal_query_seq_attn)
         return _Unpack.apply(out, q_meta)
-    return _Attention.apply(q, k, v, context_k, context_v, scale, q_meta, context_meta, causal_query_seq_attn)
+    return _Attention.apply(q, k, v, context_k, context_v, layout, scale, q_meta, context_meta, causal_query_seq_attn)
