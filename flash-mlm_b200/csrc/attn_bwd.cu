@@ -34,38 +34,51 @@ int launch_pass(const CUtensorMap* m, const BwdParams& p, cudaStream_t s) {
 }
 
 template <int D, bool KV, bool BF16>
-int run_pass(const fmlm_attn_bwd_args* a, BwdParams p, cudaStream_t s) {
+int run_pass(const CUtensorMap* m, BwdParams p, cudaStream_t s) {
   using C = BwdCfg<D, KV>;
   const long long items = (long long)(KV ? p.HK : p.H) * (p.slots + (KV ? p.cslots : 0)) * C::NDH;
   if (items > 0x7fff0000LL) return set_error(FMLM_ERR_INVALID, "problem too large");
   if (items == 0) return FMLM_OK;
   p.num_items = (int)items;
   p.counter += KV ? 1 : 0;
-  const fmlm_view4 empty = {nullptr, 0, 0, 0, 0, 0, 0};
-  const bool ctx = p.C > 0 && p.Tc > 0;
-  const int qrows = KV ? C::BN : C::BM, krows = KV ? C::BM : C::BN;
-  CUtensorMap m[6];
+  return launch_pass<D, KV, BF16>(m, p, s);
+}
+
+// Tensor maps of q, dout, k, v and the context's k, v with boxes of qrows / krows rows.
+int encode_maps(CUtensorMap* m, const fmlm_attn_bwd_args* a, bool ctx, int qrows, int krows) {
+  const int D = a->head_dim;
   int rc;
   if ((rc = encode_view(&m[0], a->q, D, qrows, a->dtype, a->q.data, "q"))) return rc;
   if ((rc = encode_view(&m[1], a->dout, D, qrows, a->dtype, a->q.data, "dout"))) return rc;
   if ((rc = encode_view(&m[2], a->k, D, krows, a->dtype, a->q.data, "k"))) return rc;
   if ((rc = encode_view(&m[3], a->v, D, krows, a->dtype, a->q.data, "v"))) return rc;
-  if ((rc = encode_view(&m[4], ctx ? a->k_context : empty, D, krows, a->dtype, a->q.data, "k_context"))) return rc;
-  if ((rc = encode_view(&m[5], ctx ? a->v_context : empty, D, krows, a->dtype, a->q.data, "v_context"))) return rc;
-  return launch_pass<D, KV, BF16>(m, p, s);
+  if (!ctx) {  // never loaded from
+    m[4] = m[2];
+    m[5] = m[3];
+    return FMLM_OK;
+  }
+  if ((rc = encode_view(&m[4], a->k_context, D, krows, a->dtype, a->q.data, "k_context"))) return rc;
+  return encode_view(&m[5], a->v_context, D, krows, a->dtype, a->q.data, "v_context");
 }
 
 template <int D, bool BF16>
 int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cudaStream_t s) {
+  using C = BwdCfg<D, false>;
   const long long vecs = rows * (D / 8);
   const long long blocks = (vecs + 255) / 256;
   if (blocks > 0x7fffffffLL) return set_error(FMLM_ERR_INVALID, "problem too large");
+  // Every map before the first launch: a refused view leaves nothing half done.
+  const bool ctx = p.C > 0;
+  CUtensorMap m[12];
+  int rc = encode_maps(m, a, ctx, C::BM, C::BN);
+  if (!rc && C::BM != C::BN) rc = encode_maps(m + 6, a, ctx, C::BN, C::BM);
+  if (rc) return rc;
   attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
       reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, rows,
       const_cast<float2*>(p.stats), p.counter);
-  int rc = check_launch("attn_bwd_stats_kernel");
-  if (!rc && a->dq) rc = run_pass<D, false, BF16>(a, p, s);
-  if (!rc && a->dk) rc = run_pass<D, true, BF16>(a, p, s);
+  rc = check_launch("attn_bwd_stats_kernel");
+  if (!rc && a->dq) rc = run_pass<D, false, BF16>(m, p, s);
+  if (!rc && a->dk) rc = run_pass<D, true, BF16>(C::BM != C::BN ? m + 6 : m, p, s);
   return rc;
 }
 
@@ -80,6 +93,8 @@ int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows
     default: return set_error(FMLM_ERR_UNSUPPORTED, "HEAD_DIM must be one of {16, 32, 64, 128, 256}");
   }
 }
+
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 int check_view(const fmlm_view4& v, const char* name, int64_t rows, int64_t heads, int64_t batch) {
   if (!v.data) return set_error(FMLM_ERR_INVALID, "%s is required", name);
@@ -131,14 +146,15 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
       return set_error(FMLM_ERR_INVALID, "a context needs cu_seqlens_context, and dk_context and dv_context with dk");
     if ((rc = check_view(a->k_context, "k_context", a->total_context_len, a->kv_heads, 1))) return rc;
     if ((rc = check_view(a->v_context, "v_context", a->total_context_len, a->kv_heads, 1))) return rc;
-    if (!aligned16(a->dk_context) || !aligned16(a->dv_context))
-      return set_error(FMLM_ERR_INVALID, "dk_context and dv_context must be 16-byte aligned");
+    if (!aligned32(a->dk_context) || !aligned32(a->dv_context))
+      return set_error(FMLM_ERR_INVALID, "dk_context and dv_context must be 32-byte aligned");
   }
   if ((a->dk == nullptr) != (a->dv == nullptr) || (!a->dq && !a->dk))
     return set_error(FMLM_ERR_INVALID, "give dq, or dk and dv, or all three");
-  if (!a->out || !a->lse || !aligned16(a->out) || !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv))
-    return set_error(FMLM_ERR_INVALID, "out and lse are required; out, dq, dk, dv must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(a->dout.data) & 15u) != 0) return set_error(FMLM_ERR_INVALID, "dout must be 16-byte aligned");
+  if (!a->out || !a->lse || !aligned16(a->out) || !aligned16(a->dout.data))
+    return set_error(FMLM_ERR_INVALID, "out and lse are required; out and dout must be 16-byte aligned");
+  if (!aligned32(a->dq) || !aligned32(a->dk) || !aligned32(a->dv))
+    return set_error(FMLM_ERR_INVALID, "dq, dk, dv must be 32-byte aligned");
   const int64_t rows = qb * a->num_heads * qr;
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < fmlm_attn_bwd_workspace_bytes(rows))
     return set_error(FMLM_ERR_INVALID, "workspace too small (%zu bytes needed)", fmlm_attn_bwd_workspace_bytes(rows));

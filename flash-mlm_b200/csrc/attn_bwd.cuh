@@ -284,6 +284,14 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   return r;
 }
 
+// One whole 32-byte sector: a thread owns a row, so neighbouring lanes write
+// far apart, and half sectors would cost the memory system twice.
+__device__ __forceinline__ void st_sector(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // 16-byte vector c of row r of a K-major tile as TMA's swizzle laid it out.
 template <int SWB>
 __device__ __forceinline__ uint4 ld_swizzled(const uint8_t* tile, int rows, int r, int c) {
@@ -435,18 +443,24 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     auto load_tile = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* b, int rows, int row, int h, int bb) {
       for (int s = 0; s < C::NSLAB; ++s) tma_load_4d(dst + s * (rows * SWB), m, b, s * C::SLAB_COLS, row, h, bb);
     };
-    auto next_item = [&]() {
-      int next = 0;
-      if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
-      w = __shfl_sync(0xffffffffu, next, 0);
-    };
-    for (uint32_t ring = 0;; ++ring) {
-      BwdItem it;
-      while (w < num_items) {
-        it = decode_bwd_item<C>(p, w, lane);
-        if (it.limit > 0) break;  // (a slot past its sequence's end writes nothing)
-        next_item();
+    // The next item that writes something, decoded (w >= num_items: none).  Its
+    // counter and offset loads take some 2000 cycles, so it is fetched before the
+    // current item's last tile is; not earlier, since a CTA in a long item
+    // would then hold back work that others are free to take (measured: a
+    // shared context's items, 72 tiles each, 202 -> 220 us).
+    BwdItem it;
+    auto fetch = [&](BwdItem& x) {
+      for (;;) {
+        if (w >= num_items) return;
+        x = decode_bwd_item<C>(p, w, lane);
+        if (x.limit > 0) return;  // (a slot past its sequence's end writes nothing)
+        int next = 0;
+        if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
+        w = __shfl_sync(0xffffffffu, next, 0);
       }
+    };
+    fetch(it);
+    for (uint32_t ring = 0;; ++ring) {
       if (!wait(&bar->item_empty[ring & 3], ((ring >> 2) & 1u) ^ 1u)) break;
       if (lane == 0) {
         if (w < num_items) ring_items[ring & 3] = it;
@@ -455,6 +469,13 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       }
       __syncwarp();
       if (w >= num_items) break;
+      BwdItem nx;
+      auto prefetch = [&]() {
+        int next = 0;
+        if (lane == 0) next = (int)gridDim.x + atomicAdd(p.counter, 1);
+        w = __shfl_sync(0xffffffffu, next, 0);
+        fetch(nx);
+      };
       const int n = it.heads * it.nt0 + it.nt1;
       if (n > 0) {
         if (!wait(&bar->a_empty, (aload & 1u) ^ 1u)) break;
@@ -509,10 +530,13 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             if (lane == 0) mbar_arrive(&bar->b1_full[st]);
           }
           if (++t == it.nt0 && KV) { t = 0; ++g; }
+          if (i + 1 == max(n - 1, 1)) prefetch();
         }
         if (failed) break;
+      } else {
+        prefetch();
       }
-      next_item();
+      it = nx;
     }
   } else if (warp == C::MMA_WARP) {
     // ------------------------------------------------------------ MMA issuer
@@ -797,16 +821,11 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           if (n > 0) tmem_ld_x16(tO + c0, o);
           if (row < limit) {
             const bool live = n > 0 && row < valid;
-            uint4* d4 = reinterpret_cast<uint4*>(dst + c0);
+            uint32_t v[8];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t v[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                v[e] = live ? pack2<BF16>(__uint_as_float(o[8 * q + 2 * e]) * f, __uint_as_float(o[8 * q + 2 * e + 1]) * f)
-                            : 0u;
-              d4[q] = make_uint4(v[0], v[1], v[2], v[3]);
-            }
+            for (int e = 0; e < 8; ++e)
+              v[e] = live ? pack2<BF16>(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f) : 0u;
+            st_sector(dst + c0, v);
           }
         }
       }

@@ -181,9 +181,9 @@ typedef struct fmlm_attn_bwd_args {
   const float* lse;                 /* the forward's lse, in the order of out's rows */
   const int32_t* cu_seqlens_q;      /* [batch + 1] (padded, packed) */
   const int32_t* cu_seqlens_context;/* [context_entries + 1] */
-  void *dq, *dk, *dv;               /* contiguous, shaped like q, k, v; padding rows get zeros.  dq may be NULL, and
+  void *dq, *dk, *dv;               /* contiguous, 32-byte aligned, shaped like q, k, v; padding rows get zeros.  dq may be NULL, and
                                        dk with dv (and the context's): gradients that nobody asks for */
-  void *dk_context, *dv_context;    /* contiguous [kv_heads][total_context_len][D]; rows of no entry are left unwritten */
+  void *dk_context, *dv_context;    /* contiguous [kv_heads][total_context_len][D], 32-byte aligned; rows of no entry are left unwritten */
   void* workspace;                  /* fmlm_attn_bwd_workspace_bytes() bytes, 16-byte aligned */
   size_t workspace_bytes;
   int32_t* error_word;
