@@ -62,7 +62,7 @@ int encode_maps(CUtensorMap* m, const fmlm_attn_bwd_args* a, bool ctx, int qrows
 }
 
 template <int D, bool BF16>
-int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cudaStream_t s) {
+int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long long rows, cudaStream_t s) {
   using C = BwdCfg<D, false>;
   const long long vecs = rows * (D / 8);
   const long long blocks = (vecs + 255) / 256;
@@ -75,7 +75,7 @@ int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cud
   if (rc) return rc;
   attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
       reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, rows,
-      const_cast<float2*>(p.stats), p.counter);
+      ext_mul, const_cast<float2*>(p.stats), const_cast<uint4*>(p.xstats), p.counter);
   rc = check_launch("attn_bwd_stats_kernel");
   if (!rc && a->dq) rc = run_pass<D, false, BF16>(m, p, s);
   if (!rc && a->dk) rc = run_pass<D, true, BF16>(C::BM != C::BN ? m + 6 : m, p, s);
@@ -83,13 +83,13 @@ int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cud
 }
 
 template <bool BF16>
-int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, long long rows, cudaStream_t s) {
+int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long long rows, cudaStream_t s) {
   switch (a->head_dim) {
-    case 16: return run_bwd<16, BF16>(a, p, rows, s);
-    case 32: return run_bwd<32, BF16>(a, p, rows, s);
-    case 64: return run_bwd<64, BF16>(a, p, rows, s);
-    case 128: return run_bwd<128, BF16>(a, p, rows, s);
-    case 256: return run_bwd<256, BF16>(a, p, rows, s);
+    case 16: return run_bwd<16, BF16>(a, p, ext_mul, rows, s);
+    case 32: return run_bwd<32, BF16>(a, p, ext_mul, rows, s);
+    case 64: return run_bwd<64, BF16>(a, p, ext_mul, rows, s);
+    case 128: return run_bwd<128, BF16>(a, p, ext_mul, rows, s);
+    case 256: return run_bwd<256, BF16>(a, p, ext_mul, rows, s);
     default: return set_error(FMLM_ERR_UNSUPPORTED, "HEAD_DIM must be one of {16, 32, 64, 128, 256}");
   }
 }
@@ -110,7 +110,7 @@ int check_view(const fmlm_view4& v, const char* name, int64_t rows, int64_t head
 using namespace fmlm;
 
 extern "C" size_t fmlm_attn_bwd_workspace_bytes(int64_t rows) {
-  return kCounterBytes + (size_t)(rows > 0 ? rows : 0) * sizeof(float2);
+  return kCounterBytes + (size_t)(rows > 0 ? rows : 0) * (sizeof(float2) + sizeof(uint4));
 }
 
 extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
@@ -177,7 +177,8 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.cu_q = a->cu_seqlens_q;
   p.cu_c = a->cu_seqlens_context;
   p.counter = reinterpret_cast<int*>(a->workspace);
-  p.stats = reinterpret_cast<const float2*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
+  p.xstats = reinterpret_cast<const uint4*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
+  p.stats = reinterpret_cast<const float2*>(p.xstats + rows);
   p.dq = a->dq;
   p.dk = a->dk;
   p.dv = a->dv;
@@ -193,9 +194,14 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   // what the 16-bit columns hold is of lse's own magnitude.
   const int e = std::min(15, std::max(-14, -std::ilogb(p.scale_log2)));
   p.ext_unit = std::ldexp(1.f, e);
-  p.ext_mul = 1.f / (p.scale_log2 * p.ext_unit);
+  const float ext_mul = 1.f / (p.scale_log2 * p.ext_unit);
+  // -400 in the exponent; one 16-bit number is near enough
+  const float none = -400.f * ext_mul;
+  p.xnone = make_uint4(a->dtype == FMLM_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(none))
+                                                   : __half_as_ushort(__float2half_rn(none)), 0, 0, 0);
   p.err = a->error_word;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == FMLM_DTYPE_BF16 ? dispatch_bwd<true>(a, p, rows, s) : dispatch_bwd<false>(a, p, rows, s);
+  return a->dtype == FMLM_DTYPE_BF16 ? dispatch_bwd<true>(a, p, ext_mul, rows, s)
+                                     : dispatch_bwd<false>(a, p, ext_mul, rows, s);
 }

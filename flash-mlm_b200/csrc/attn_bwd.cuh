@@ -26,7 +26,8 @@
 //
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
-// warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs.
+// warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs,
+// warp 18 (KV) copies the streamed rows' extra columns.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -47,11 +48,12 @@ struct BwdParams {
   const int* cu_q;
   const int* cu_c;
   const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta}
+  const uint4* xstats;  // the same as what the KV pass puts into B's extra columns
+  uint4 xnone;          // xstats of a row that is not there: P = 2^-400 = 0, delta = 0
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
   float scale, scale_log2;  // scale_log2: of the scores in the exponent (never 0: see the host code)
   float ext_unit;           // KV: A's constant (a power of two) for the lse columns
-  float ext_mul;            // KV: 1 / (scale_log2 * ext_unit)
   int* err;
   unsigned long long timeout_ns;
 };
@@ -82,7 +84,8 @@ struct BwdCfg {
   static constexpr int EW_WARPS = 4 * EW_GROUPS;
   static constexpr int TMA_WARP = EW_WARPS;
   static constexpr int MMA_WARP = EW_WARPS + 1;
-  static constexpr int THREADS = 32 * (EW_WARPS + 2);
+  static constexpr int EXT_WARP = EW_WARPS + 2;
+  static constexpr int THREADS = 32 * (EW_WARPS + (KV ? 3 : 2));
   static constexpr int NC = BN / EW_GROUPS;  // score columns per element-wise warp
   static constexpr int TM_S = 0, TM_DP = BN, TM_P = SEP_P ? 2 * BN : 0;
   static constexpr int TM_ACC1 = 2 * BN + (SEP_P ? BN / 2 : 0), TM_ACC2 = TM_ACC1 + (KV ? DV : 0);
@@ -338,6 +341,15 @@ __device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
   if constexpr (!BF16) c = fminf(fmaxf(c, -65504.f), 65504.f);
 }
 
+// The extra columns of a row: three of B1 (lse) in x, y; three of B2 (delta) in z, w.
+template <bool BF16>
+__device__ __forceinline__ uint4 ext_columns(float nl, float nd) {
+  float a, b, c, d, e, f;
+  split3<BF16>(nl, a, b, c);
+  split3<BF16>(nd, d, e, f);
+  return make_uint4(pack2<BF16>(a, b), pack2<BF16>(c, 0.f), pack2<BF16>(0.f, d), pack2<BF16>(e, f));
+}
+
 template <int D, bool KV, bool BF16>
 __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
@@ -369,7 +381,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       mbar_init(&bar->b1_empty[i], 1);
       mbar_init(&bar->b2_empty[i], 1);
       mbar_init(&bar->item_full[i], 1);
-      mbar_init(&bar->item_empty[i], C::EW_WARPS + 1);
+      mbar_init(&bar->item_empty[i], C::EW_WARPS + (KV ? 2 : 1));
     }
     mbar_init(&bar->s_full, 1);
     mbar_init(&bar->dp_full, 1);
@@ -494,7 +506,6 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           const uint32_t ph = (fill / STAGES) & 1u;
           const bool second = !KV && t >= it.nt0;
           const int row = second ? it.row1 + (t - it.nt0) * BN : it.row0 + t * BN;
-          const int end = second ? it.end1 : it.end0;
           const int h = it.h0 + g;
           const bool cmap = !KV && it.map0 == 1 && !second;
           uint8_t* d1 = sB + st * 2 * C::B_BYTES;
@@ -510,25 +521,6 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             load_tile(d1 + C::B_BYTES, KV ? &tm_do : cmap ? &tm_vc : &tm_v, &bar->b2_full[st], BN, row, h, it.b);
           }
           __syncwarp();
-          if constexpr (KV) {
-            // The streamed rows' extra columns; rows past the range (their
-            // tile rows are cleared: S = dP = 0) get P = 2^-400 = 0.
-            const float2* src = p.stats + it.stat0 + (long long)g * it.stat_h;
-            uint8_t* x1 = sBx + st * 2 * C::BX_BYTES;
-#pragma unroll
-            for (int c = lane; c < BN; c += 32) {
-              const float2 x = row + c < end ? __ldg(src + row + c) : make_float2(-400.f, 0.f);
-              float u, v, w;
-              split3<BF16>(x.x * p.ext_mul, u, v, w);
-              *reinterpret_cast<uint4*>(ext_row(x1, c, 0)) = make_uint4(pack2<BF16>(u, v), pack2<BF16>(w, 0.f), 0, 0);
-              split3<BF16>(x.y, u, v, w);
-              *reinterpret_cast<uint4*>(ext_row(x1 + C::BX_BYTES, c, 0)) =
-                  make_uint4(0, pack2<BF16>(0.f, u), pack2<BF16>(v, w), 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar->b1_full[st]);
-          }
           if (++t == it.nt0 && KV) { t = 0; ++g; }
           if (i + 1 == max(n - 1, 1)) prefetch();
         }
@@ -537,6 +529,46 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         prefetch();
       }
       it = nx;
+    }
+  } else if (KV && warp == C::EXT_WARP) {
+    // ------------------------------------------------------------ extra columns
+    // Loaded one tile ahead: the stage is waited for with the values in hand.
+    uint32_t fill = 0;
+    for (uint32_t ring = 0;; ++ring) {
+      const BwdItem* slot = take_item(ring);
+      if (!slot) break;
+      const int nt0 = slot->nt0, n = slot->heads * nt0, row0 = slot->row0, end0 = slot->end0, stat_h = slot->stat_h;
+      const uint4* src = p.xstats + slot->stat0;
+      release_item(ring);
+      uint4 x[BN / 32];
+      int t = 0;
+      auto load = [&]() {  // tile t of the head at src, and on to the next
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          const int r = row0 + t * BN + c * 32 + lane;
+          x[c] = r < end0 ? __ldg(src + r) : p.xnone;
+        }
+        if (++t == nt0) {
+          t = 0;
+          src += stat_h;
+        }
+      };
+      if (n > 0) load();
+      for (int i = 0; i < n; ++i, ++fill) {
+        const int st = fill % STAGES;
+        if (!wait(&bar->b1_empty[st], ((fill / STAGES) & 1u) ^ 1u)) break;
+        uint8_t* x1 = sBx + st * 2 * C::BX_BYTES;
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          *reinterpret_cast<uint4*>(ext_row(x1, c * 32 + lane, 0)) = make_uint4(x[c].x, x[c].y, 0, 0);
+          *reinterpret_cast<uint4*>(ext_row(x1 + C::BX_BYTES, c * 32 + lane, 0)) = make_uint4(0, x[c].z, x[c].w, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->b1_full[st]);
+        if (i + 1 < n) load();
+      }
+      if (failed) break;
     }
   } else if (warp == C::MMA_WARP) {
     // ------------------------------------------------------------ MMA issuer
@@ -849,8 +881,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   }
 }
 
-// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}; also
-// zeroes the item counters of the two passes that follow.  Reads O and dO
+// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}, in float32 and as
+// the KV pass's extra columns; also zeroes the item counters of the two passes that follow.  Reads O and dO
 // once (bound by HBM).  delta uses the 16-bit O that the forward pass returned:
 // its rounding (half a step per element) enters dS as |dO| * 2^-9 noise, below
 // that of dS's own rounding to 16 bits.
@@ -858,7 +890,8 @@ template <int D, bool BF16>
 __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const uint4* __restrict__ out,
                                                              const uint4* __restrict__ dout,
                                                              const float* __restrict__ lse, long long rows,
-                                                             float2* __restrict__ stats, int* counters) {
+                                                             float ext_mul, float2* __restrict__ stats,
+                                                             uint4* __restrict__ xstats, int* counters) {
   constexpr int LANES = D / 8;  // 16-byte vectors per row
   if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -882,8 +915,11 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const uint4* __rest
   }
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (r < rows && threadIdx.x % LANES == 0)
-    stats[r] = make_float2(fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp), -s);
+  if (r < rows && threadIdx.x % LANES == 0) {
+    const float nl = fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp);
+    stats[r] = make_float2(nl, -s);
+    xstats[r] = ext_columns<BF16>(nl * ext_mul, -s);
+  }
 }
 
 }  // namespace fmlm
