@@ -289,7 +289,7 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 
 // One whole 32-byte sector: a thread owns a row, so neighbouring lanes write
 // far apart, and half sectors would cost the memory system twice.
-__device__ __forceinline__ void st_sector(void* p, const uint32_t (&v)[8]) {
+__device__ __forceinline__ void st_sector(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
@@ -769,6 +769,25 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       if (lane == 0) mbar_arrive(&bar->a_empty);
       return true;
     };
+    // Results wait in registers (16-bit pairs) until the next item's first
+    // scores are in hand: their stores then drain behind its exponentials
+    // instead of in front of them (up to 32 columns; 64, in 32 registers, lost
+    // at D = 128: KV pass 123 -> 131 us).  KV: groups 0, 1 hold halves of dV, groups
+    // 2, 3 halves of dK; Q: quarters of dQ.
+    constexpr int PARTS = KV ? 2 : 4;
+    constexpr int COLS = C::DV / PARTS >= 16 ? C::DV / PARTS : 16;
+    constexpr bool kDefer = COLS <= 32;
+    const int part = KV ? g & 1 : g;
+    const bool is_dv = KV && g < 2;
+    uint32_t res[COLS / 2];
+    T* res_dst = nullptr;
+    auto flush = [&]() {
+      if (res_dst != nullptr) {
+#pragma unroll
+        for (int c = 0; c < COLS / 16; ++c) st_sector(res_dst + c * 16, res + 8 * c);
+      }
+      res_dst = nullptr;
+    };
     const BwdItem* it = take_item(0);
     if (C::ATM && it && it->heads * it->nt0 + it->nt1 > 0 && !copy_a()) it = nullptr;
     for (uint32_t ring = 0; it; ++ring) {
@@ -776,13 +795,15 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
       const F2 nl_2 = f2(rs.x, rs.x), nd_2 = f2(rs.y * kInv, rs.y * kInv);
-      for (int i = 0; i < n; ++i, ph ^= 1u) {
-        if (!wait(&bar->s_full, ph)) break;
+      // (the first tile apart, so that the waiting results leave their registers there)
+      auto tile = [&](auto first, int i) -> bool {
+        if (!wait(&bar->s_full, ph)) return false;
         tc_fence_after();
         uint32_t x[NC];
         F2 pr[NC / 2];
         ld(tS, x);
         if (C::SEP_P || !KV) arrive(&bar->s_free);
+        if constexpr (kDefer && decltype(first)::value) flush();
 #pragma unroll
         for (int c = 0; c < NC / 2; ++c) {
           const F2 xs = f2u(x[2 * c], x[2 * c + 1]);
@@ -795,7 +816,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
 #pragma unroll
           for (int c = 0; c < NC / 2; ++c) pk[c] = pack2<BF16>(pr[c]);
           if (C::SEP_P) {
-            if (!wait(&bar->p_free, ph ^ 1u)) break;
+            if (!wait(&bar->p_free, ph ^ 1u)) return false;
             tc_fence_after();
           }
           st16(tP, pk);
@@ -811,7 +832,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             }
           }
         }
-        if (!wait(&bar->dp_full, ph)) break;
+        if (!wait(&bar->dp_full, ph)) return false;
         tc_fence_after();
         ld(tDP, x);
 #pragma unroll
@@ -823,45 +844,49 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         }
         st16(tDP, pk);
         arrive(&bar->ds_full);
-      }
+        ph ^= 1u;
+        return true;
+      };
+      if (n > 0 && tile(std::true_type(), 0))
+        for (int i = 1; i < n && tile(std::false_type(), i); ++i) {}
       if (failed) break;
+      // dP of the last tile was the last MMA to read the stationary tiles (and
+      // came after the last S), so the next item's can move in: its first
+      // scores follow this item's last accumulations at once.
+      const BwdItem* next = take_item(ring + 1);
+      if (failed) break;
+      const int next_n = next ? next->heads * next->nt0 + next->nt1 : 0;
+      if (C::ATM && next_n > 0 && !copy_a()) break;
+      const int valid = it->valid, limit = it->limit;
+      if (part * COLS < C::DV && row < limit) {
+        T* base = reinterpret_cast<T*>(!KV ? p.dq : is_dv ? (it->a_map ? p.dvc : p.dv) : (it->a_map ? p.dkc : p.dk));
+        res_dst = base + (it->out_row + row) * (long long)D + it->dh * C::DV + part * COLS;
+      }
       if (n > 0) {
         if (!wait(&bar->acc_full, acc_ph)) break;
         acc_ph ^= 1u;
         tc_fence_after();
-      }
-      // Every MMA of this item is done, so the next item's stationary tiles
-      // can move in before the epilogue: its first scores run during it.
-      const BwdItem* next = take_item(ring + 1);
-      if (failed) break;
-      if (C::ATM && next && next->heads * next->nt0 + next->nt1 > 0 && !copy_a()) break;
-      // epilogue: accumulators -> global, a quarter of the columns per warp group
-      // (KV: groups 0, 1 halves of dV, groups 2, 3 halves of dK)
-      constexpr int PARTS = KV ? 2 : 4;
-      constexpr int COLS = C::DV / PARTS >= 16 ? C::DV / PARTS : 16;
-      const int part = KV ? g & 1 : g;
-      if (part * COLS < C::DV) {
-        const bool is_dv = KV && g < 2;
-        const uint32_t tO = tmem_base + lane_off + (is_dv ? C::TM_ACC1 : C::TM_ACC2) + part * COLS;
-        const float f = is_dv ? kInv : p.scale;
-        const int valid = it->valid, limit = it->limit;
-        T* base = reinterpret_cast<T*>(!KV ? p.dq : is_dv ? (it->a_map ? p.dvc : p.dv) : (it->a_map ? p.dkc : p.dk));
-        T* dst = base + (it->out_row + row) * (long long)D + it->dh * C::DV + part * COLS;
-#pragma unroll 1
-        for (int c0 = 0; c0 < COLS; c0 += 16) {
-          uint32_t o[16];
-          if (n > 0) tmem_ld_x16(tO + c0, o);
-          if (row < limit) {
-            const bool live = n > 0 && row < valid;
-            uint32_t v[8];
+        if (part * COLS < C::DV) {
+          const uint32_t tO = tmem_base + lane_off + (is_dv ? C::TM_ACC1 : C::TM_ACC2) + part * COLS;
+          const float fs = is_dv ? kInv : p.scale;
+          const F2 f = f2(fs, fs);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[e] = live ? pack2<BF16>(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f) : 0u;
-            st_sector(dst + c0, v);
+          for (int c0 = 0; c0 < COLS; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld_x16(tO + c0, o);
+            const int at = kDefer ? c0 / 2 : 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) res[at + e] = row < valid ? pack2<BF16>(mul2(f2u(o[2 * e], o[2 * e + 1]), f)) : 0u;
+            if (!kDefer && res_dst != nullptr) st_sector(res_dst + c0, res);
           }
         }
+        if (!kDefer) res_dst = nullptr;
+        arrive(&bar->acc_empty);
+      } else {
+#pragma unroll
+        for (int e = 0; e < COLS / 2; ++e) res[e] = 0u;
       }
-      if (n > 0) arrive(&bar->acc_empty);
+      if (next_n == 0 || !kDefer) flush();
       release_item(ring);
       it = next;
     }
