@@ -141,12 +141,19 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   auto tiles = [](int r0, int r1) { return r1 > r0 ? (r1 - r0 + BN - 1) / BN : 0; };
   it.dh = w % C::NDH;
   w /= C::NDH;
-  // KV: the context's slots first (a shared context streams the whole batch past: the longest items)
-  const int per_head = p.slots + (C::KV ? p.cslots : 0);
-  const int h = w / per_head;
-  int v = w % per_head;
+  // Heads fastest, and the longest items first, so that none is left for the
+  // end: the context's (a shared one streams the whole batch past) before the
+  // sequences', and with causal_query_seq_attn the sequences with most to
+  // stream (KV pass: the first, Q pass: the last) before the others.
+  // Sequences of one length (dense) go head by head instead, whose streamed
+  // tiles then stay in L2 (16 heads of 8192 x 128: KV 793 -> 768, Q 649 -> 628 us).
+  const int heads = C::KV ? p.HK : p.H;
+  const bool dense = p.layout == FMLM_BWD_DENSE;
+  const int h = dense ? w / p.slots : w % heads;
+  int v = dense ? w % p.slots : w / heads;
   const bool ctx = C::KV && v < p.cslots;
   if (C::KV && !ctx) v -= p.cslots;
+  if (!C::KV && p.causal) v = p.slots - 1 - v;
   const bool packed = p.layout == FMLM_BWD_PACKED;
   it.map0 = 0; it.row1 = it.end1 = it.nt1 = 0;
   it.a_map = ctx ? 1 : 0;
