@@ -164,7 +164,8 @@ def _args(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, p
 
 
 def _outputs(q, k):
-    return (torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    return (torch.empty_like(q, memory_format=torch.contiguous_format),
+            torch.empty_like(k, memory_format=torch.contiguous_format))
 
 
 def _forward(q, k, *call):
@@ -194,7 +195,7 @@ def _rope_backward(ctx, gq, gk):
     q, k, q_weight, k_weight, positions, position_offsets = ctx.saved_tensors
     rotary, normalize, eps, q_meta = ctx.call
     dq, dk = _outputs(q, k)
-    dwq, dwk = (torch.empty(w.shape, dtype=w.dtype, device=w.device) if w is not None and need else None
+    dwq, dwk = (torch.empty_like(w, memory_format=torch.contiguous_format) if w is not None and need else None
                 for w, need in ((q_weight, ctx.needs_input_grad[2]), (k_weight, ctx.needs_input_grad[3])))
     if not (q.numel() and k.numel()):
         for w in (dwq, dwk):

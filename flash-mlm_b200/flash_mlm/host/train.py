@@ -148,7 +148,7 @@ def flash_attn_mlm_fwd(
 
 def _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta, causal):
     """``flash_attn_mlm_fwd`` on checked arguments."""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
     if _nothing_to_do(q, q_meta):
         return out.zero_(), lse.fill_(float("-inf"))
@@ -232,7 +232,7 @@ def _backward(layout, dout, q, k, v, out, lse, scale, q_meta, context_k, context
     dev = q.device
 
     def like(x, wanted):
-        return torch.empty(x.shape, dtype=x.dtype, device=dev) if wanted and x is not None else None
+        return torch.empty_like(x, memory_format=torch.contiguous_format) if wanted and x is not None else None
 
     dq, dk, dv = like(q, need_dq), like(k, need_dkv), like(v, need_dkv)
     dkc, dvc = like(context_k, need_dkv), like(context_v, need_dkv)
