@@ -12,6 +12,13 @@
 // row sums are shuffles over those lanes.  A lane group walks the heads of one
 // token, so the token's cosines and sines, which are the same for every head,
 // are loaded once.  All arithmetic is in 32 bits; outputs are rounded once.
+//
+// What keeps memory busy is the loads that each thread has under way: four
+// heads at a time forward, two backward, and the registers for them rather than
+// more warps.  16 x 4096 tokens, 32 + 8 heads of 128, a projection's strides:
+// forward 227 us (5.9 TB/s; with registers capped for two blocks per SM 254,
+// two heads at a time 268, eight 282), backward 400 us (5.0 TB/s; one head at a
+// time and three blocks 445, weights in registers 439).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -199,7 +206,7 @@ __device__ __forceinline__ float row_sum(float s) {
 }
 
 template <int D, bool HALF, bool BF16>
-__global__ void __launch_bounds__(kThreads) qk_rope_fwd_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kThreads, 1) qk_rope_fwd_kernel(const RopeParams p) {
   constexpr int LPR = D / 16, UNROLL = 4;
   const int l = threadIdx.x % LPR;
   const long long i = (long long)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) qk_rope_fwd_kernel(const RopeParams 
 // Blocks walk token tiles with a stride of the grid, keeping their share of
 // the weights' gradient in registers; each ends with one row of partial sums.
 template <int D, bool HALF, bool BF16>
-__global__ void __launch_bounds__(kThreads) qk_rope_bwd_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kThreads, 2) qk_rope_bwd_kernel(const RopeParams p) {
   constexpr int LPR = D / 16, UNROLL = 2, TOK = kThreads / LPR;
   __shared__ float red[kThreads / 32][D];
   const int l = threadIdx.x % LPR;
@@ -264,8 +271,17 @@ __global__ void __launch_bounds__(kThreads) qk_rope_bwd_kernel(const RopeParams 
   const int h1 = min(h0 + p.head_step, p.heads[which]);
   int c0, c1;
   lane_columns(p.R, l, c0, c1);
-  float w[16], dw[16];
-  load_weights<BF16>(p, p.w[which], c0, c1, w);
+  // the lanes' weights in shared memory (rows of 80 bytes: no two lanes of a
+  // row on the same bank): 16 registers fewer than holding them
+  __shared__ float4 sw[LPR][5];
+  if (threadIdx.x < LPR) {
+    float w0[16];
+    load_weights<BF16>(p, p.w[which], c0, c1, w0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sw[l][e] = make_float4(w0[4 * e], w0[4 * e + 1], w0[4 * e + 2], w0[4 * e + 3]);
+  }
+  __syncthreads();
+  float dw[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) dw[e] = 0.f;
   const long long sh = p.xs[which][1], gh = p.gs[which][1];
@@ -305,6 +321,12 @@ __global__ void __launch_bounds__(kThreads) qk_rope_bwd_kernel(const RopeParams 
         if (p.normalize) {
           unpack8<BF16>(a[u], v);
           unpack8<BF16>(b[u], v + 8);
+          float w[16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 x4 = sw[l][e];
+            w[4 * e] = x4.x; w[4 * e + 1] = x4.y; w[4 * e + 2] = x4.z; w[4 * e + 3] = x4.w;
+          }
           float s = 0.f, c = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
