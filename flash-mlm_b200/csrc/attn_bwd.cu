@@ -75,9 +75,11 @@ int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long
   if (rc) return rc;
   attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
       reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, rows,
-      ext_mul, const_cast<float2*>(p.stats), const_cast<uint4*>(p.xstats), p.counter);
+      ext_mul, const_cast<float2*>(p.stats), p.xstats, p.counter);
   rc = check_launch("attn_bwd_stats_kernel");
-  if (!rc && a->dq) rc = run_pass<D, false, BF16>(m, p, s);
+  // Without dq the Q pass still leaves short rows' delta for the KV pass (where
+  // there can be such rows).
+  if (!rc && (a->dq || a->layout != FMLM_BWD_DENSE || a->seq_len <= C::BN)) rc = run_pass<D, false, BF16>(m, p, s);
   if (!rc && a->dk) rc = run_pass<D, true, BF16>(C::BM != C::BN ? m + 6 : m, p, s);
   return rc;
 }
@@ -177,7 +179,7 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.cu_q = a->cu_seqlens_q;
   p.cu_c = a->cu_seqlens_context;
   p.counter = reinterpret_cast<int*>(a->workspace);
-  p.xstats = reinterpret_cast<const uint4*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
+  p.xstats = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
   p.stats = reinterpret_cast<const float2*>(p.xstats + rows);
   p.dq = a->dq;
   p.dk = a->dk;

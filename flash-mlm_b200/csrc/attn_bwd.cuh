@@ -24,6 +24,13 @@
 // units of the scores) and -delta as sums of three 16-bit numbers, A the
 // matching constants, so S and dP arrive with them subtracted.
 //
+// delta is dO * O with O as the forward pass returned it, in 16 bits.  Over many
+// keys that costs little (dq, dk within 1.5 of the error of gradients that are
+// only rounded at the end), but not over a few, where O is as large as v: two
+// keys, 2.4.  So a Q item whose keys fit one tile (or are at most 64 in two
+// ranges, which it then walks twice) sums delta = sum_k P dP itself, in 32 bits
+// (1.4), and leaves it for the KV pass, which runs after.
+//
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
 // warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs,
@@ -48,7 +55,7 @@ struct BwdParams {
   const int* cu_q;
   const int* cu_c;
   const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta}
-  const uint4* xstats;  // the same as what the KV pass puts into B's extra columns
+  uint4* xstats;        // the same as what the KV pass puts into B's extra columns
   uint4 xnone;          // xstats of a row that is not there: P = 2^-400 = 0, delta = 0
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
@@ -103,9 +110,11 @@ struct BwdCfg {
   static constexpr int AX_BYTES = KV ? BM * 32 : 0;
   static constexpr int BX_BYTES = KV ? BN * 32 : 0;
   static constexpr int SMEM_TILES = 2 * A_BYTES + 2 * STAGES * B_BYTES + AX_BYTES + 2 * STAGES * BX_BYTES;
+  static constexpr int SUM_BYTES = KV ? 0 : 2 * EW_GROUPS * BM * 4;  // Q: delta's partial sums, twice
+  static constexpr int EXACT_KEYS = 64;  // Q: items of several tiles with at most so many keys sum delta themselves
   static constexpr int RING = 4;
   static constexpr int ITEM_BYTES = 96;
-  static constexpr int SMEM_BYTES = SMEM_TILES + 512 + RING * ITEM_BYTES + 1024;
+  static constexpr int SMEM_BYTES = SMEM_TILES + 512 + RING * ITEM_BYTES + SUM_BYTES + 1024;
 };
 
 // A work item: the stationary tile, the rows it writes and up to two ranges of
@@ -118,6 +127,7 @@ struct BwdItem {
   int map0, row0, end0, nt0;   // first range (context when map0 = 1)
   int row1, end1, nt1;         // second range (main)
   int stat_h;                  // KV: stats rows of one streamed head
+  int pre;                     // Q: tiles walked first for delta alone (0 or all of them)
   long long out_row;           // output row of the tile's row 0 (also its stats row in the Q pass)
   long long stat0;             // KV: stats row of (head h0, streamed row 0)
 };
@@ -219,6 +229,13 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   if (C::KV) it.stat0 = ((long long)(packed ? 0 : it.b) * p.H + it.h0) * it.stat_h;
   it.nt0 = tiles(it.row0, it.end0);
   if (it.valid == 0) it.nt0 = it.nt1 = 0;
+  it.pre = 0;
+  if constexpr (!C::KV) {
+    const int n = it.nt0 + it.nt1, keys = max(it.end0 - it.row0, 0) + max(it.end1 - it.row1, 0);
+    if (n > 1 && keys <= C::EXACT_KEYS) it.pre = n;
+    // dq not asked for: only items that have a delta to leave
+    if (p.dq == nullptr && n != 1 && it.pre == 0) it.valid = it.limit = it.nt0 = it.nt1 = 0;
+  }
   return it;
 }
 
@@ -230,6 +247,7 @@ struct __align__(8) BwdBarriers {
   uint64_t s_free;            // element-wise -> MMA: S is in registers
   uint64_t p_full[2], ds_full[2];  // element-wise -> MMA: P / dS written (or its first, second half)
   uint64_t p_free;            // MMA -> element-wise (separate P): P consumed
+  uint64_t sum_full;          // Q: every warp's part of delta is in shared memory
   uint64_t acc_full, acc_empty;
   uint64_t item_full[4], item_empty[4];
   int item_idx[4];
@@ -380,6 +398,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   uint8_t* sBx = sAx + C::AX_BYTES;             // KV: [STAGES][B1's, B2's extra columns]
   BwdBarriers* bar = reinterpret_cast<BwdBarriers*>(smem + C::SMEM_TILES);
   BwdItem* ring_items = reinterpret_cast<BwdItem*>(reinterpret_cast<uint8_t*>(bar) + 512);
+  float* sSum = reinterpret_cast<float*>(ring_items + C::RING);  // Q: [2][EW_GROUPS][BM]
   volatile int* abort_flag = &bar->abort_flag;
 
   const int warp = threadIdx.x >> 5;
@@ -405,6 +424,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       mbar_init(&bar->p_full[i], C::EW_WARPS);
       mbar_init(&bar->ds_full[i], C::EW_WARPS);
     }
+    mbar_init(&bar->sum_full, C::EW_WARPS);
     mbar_init(&bar->acc_full, 1);
     mbar_init(&bar->acc_empty, C::EW_WARPS);
     bar->abort_flag = 0;
@@ -503,7 +523,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         w = __shfl_sync(0xffffffffu, next, 0);
         fetch(nx);
       };
-      const int n = it.heads * it.nt0 + it.nt1;
+      const int n = it.heads * it.nt0 + it.nt1 + it.pre;
       if (n > 0) {
         if (!wait(&bar->a_empty, (aload & 1u) ^ 1u)) break;
         if (lane == 0) {
@@ -536,7 +556,9 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             load_tile(d1 + C::B_BYTES, KV ? &tm_do : cmap ? &tm_vc : &tm_v, &bar->b2_full[st], BN, row, h, it.b);
           }
           __syncwarp();
-          if (++t == it.nt0 && KV) { t = 0; ++g; }
+          ++t;
+          if (KV && t == it.nt0) { t = 0; ++g; }
+          if (!KV && t == it.nt0 + it.nt1) t = 0;  // (after the walk for delta)
           if (i + 1 == max(n - 1, 1)) prefetch();
         }
         if (failed) break;
@@ -669,7 +691,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     for (uint32_t ring = 0;; ++ring) {
       const BwdItem* slot = take_item(ring);
       if (!slot) break;
-      const int nt0 = slot->nt0, nt1 = slot->nt1, n = slot->heads * nt0 + nt1;
+      const int nt0 = slot->nt0, nt1 = slot->nt1, pre = KV ? 0 : slot->pre, n = slot->heads * nt0 + nt1 + pre;
       // valid rows of each range's last tile
       const int last0 = slot->end0 - slot->row0 - (nt0 - 1) * BN, last1 = slot->end1 - slot->row1 - (nt1 - 1) * BN;
       const uint32_t dh_off = (slot->dh * C::DV / C::SLAB_COLS) * (BN * SWB);
@@ -677,15 +699,21 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       if (n == 0) continue;
       if (!wait(C::ATM ? &bar->a_tm : &bar->a_full, aload & 1u)) break;
       ++aload;
-      // Tiles left in the range that S / dP walk, and that range's last tile.
+      // Tiles left in the range that S / dP walk (KV: its one range, once per
+      // head; Q: one range, or the two in turn), and that range's last tile.
       int s_left = nt0 > 0 ? nt0 : nt1, d_left = s_left;
       int s_last = nt0 > 0 ? last0 : last1, d_last = s_last;
+      bool s_second = nt0 == 0, d_second = s_second;
+      auto next_range = [&](bool& second, int& left, int& last) {
+        if (!KV) second = second ? nt0 == 0 : nt1 > 0;
+        left = second ? nt1 : nt0;
+        last = second ? last1 : last0;
+      };
       auto do_s = [&]() -> bool {
         if (!wait(&bar->b1_full[s_st.i], s_st.ph)) return false;
         if (--s_left == 0) {
           if (s_last < BN) clear_rows(sB + s_st.i * 2 * C::B_BYTES, s_last);
-          s_left = KV ? nt0 : nt1;
-          if (!KV) s_last = last1;
+          next_range(s_second, s_left, s_last);
         }
         tc_fence_after();
         issue_scores(tmem_base + C::TM_S, tmem_base + C::TM_A1, a1, sB0 + s_st.i * 2 * C::B_BYTES,
@@ -697,8 +725,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         if (!wait(&bar->b2_full[d_st.i], d_st.ph)) return false;
         if (--d_left == 0) {
           if (d_last < BN) clear_rows(sB + d_st.i * 2 * C::B_BYTES + C::B_BYTES, d_last);
-          d_left = KV ? nt0 : nt1;
-          if (!KV) d_last = last1;
+          next_range(d_second, d_left, d_last);
         }
         tc_fence_after();
         issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + d_st.i * 2 * C::B_BYTES + C::B_BYTES,
@@ -710,7 +737,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       if (!do_s() || !do_dp()) break;
       bool ok = true;
       for (int left = n; left > 0; --left, ph ^= 1u) {
-        const bool more = left > 1, first = left == n;
+        const bool more = left > 1, first = left == n - pre;  // (first to accumulate)
         const uint32_t b1 = sB0 + c_st.i * 2 * C::B_BYTES + dh_off, b2 = b1 + C::B_BYTES;
         if (!C::ATM && !more) commit(&bar->a_empty);  // every S and dP of the item is issued
         // The next S as soon as its columns are free: this S is in registers,
@@ -730,8 +757,14 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           if (C::SEP_P) commit(&bar->p_free);
         }
         if (!kEarlyS && STAGES > 1 && more && !do_s()) { ok = false; break; }
-        if (!issue_acc(bar->ds_full, ph, tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1, !first,
-                       &bar->b1_empty[c_st.i])) { ok = false; break; }
+        if (!KV && left > n - pre) {  // delta only: dP is read, B1 is free
+          if (!wait(bar->ds_full, ph)) { ok = false; break; }
+          commit(&bar->b1_empty[c_st.i]);
+        } else if (!issue_acc(bar->ds_full, ph, tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1, !first,
+                              &bar->b1_empty[c_st.i])) {
+          ok = false;
+          break;
+        }
         c_st.next();
         if (more) {
           if ((STAGES == 1 && !do_s()) || !do_dp()) { ok = false; break; }
@@ -752,7 +785,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
     constexpr float kInv = BwdScale<BF16>::kInv;
     const F2 sl2_2 = f2(p.scale_log2, p.scale_log2), kinv_2 = f2(kInv, kInv);
-    uint32_t ph = 0, acc_ph = 0, aload = 0;
+    uint32_t ph = 0, acc_ph = 0, aload = 0, sums = 0;
     auto arrive = [&](uint64_t* b) {
       tc_fence_before();
       __syncwarp();
@@ -817,12 +850,14 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const BwdItem* it = take_item(0);
     if (C::ATM && it && it->heads * it->nt0 + it->nt1 > 0 && !copy_a()) it = nullptr;
     for (uint32_t ring = 0; it; ++ring) {
-      const int nt0 = it->nt0, n = it->heads * nt0 + it->nt1;
+      const int nt0 = it->nt0, pre = KV ? 0 : it->pre, n = it->heads * nt0 + it->nt1 + pre;
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
-      const F2 nl_2 = f2(rs.x, rs.x), nd_2 = f2(rs.y * kInv, rs.y * kInv);
-      // (the first tile apart, so that the waiting results leave their registers there)
-      auto tile = [&](auto first, int i) -> bool {
+      const F2 nl_2 = f2(rs.x, rs.x);
+      F2 nd_2 = f2(rs.y * kInv, rs.y * kInv);
+      // (The first tile apart, so that the waiting results leave their registers
+      // there; and apart the items that sum delta themselves.)
+      auto tile = [&](auto first, auto exact, int i) -> bool {
         if (!wait(&bar->s_full, ph)) return false;
         tc_fence_after();
         uint32_t x[NC];
@@ -851,7 +886,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           }
         }
         if constexpr (!KV) {
-          const int valid = (i >= nt0 ? it->end1 - (it->row1 + (i - nt0) * BN) : it->end0 - (it->row0 + i * BN)) - g * NC;
+          const int j = decltype(exact)::value && i >= pre ? i - pre : i;
+          const int valid = (j >= nt0 ? it->end1 - (it->row1 + (j - nt0) * BN) : it->end0 - (it->row0 + j * BN)) - g * NC;
           if (valid < NC) {
 #pragma unroll
             for (int c = 0; c < NC / 2; ++c) {
@@ -864,6 +900,35 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         if (!wait(&bar->dp_full, ph)) return false;
         tc_fence_after();
         ld(tDP, x);
+        if constexpr (!KV && decltype(exact)::value) {
+          if (i < pre || n == 1) {
+            F2 acc = f2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) acc = fma2(pr[c], f2u(x[2 * c], x[2 * c + 1]), acc);
+            float a, b;
+            unf2(acc, a, b);
+            float* part = sSum + (sums & 1u) * (C::EW_GROUPS * C::BM) + row;
+            part[g * C::BM] = i == 0 ? a + b : part[g * C::BM] + (a + b);
+            if (i == pre - 1 || n == 1) {
+              // The four column groups' parts, in the same order by all.
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar->sum_full);
+              if (!wait(&bar->sum_full, sums & 1u)) return false;
+              ++sums;
+              const float nd = -((part[0] + part[C::BM]) + (part[2 * C::BM] + part[3 * C::BM])) * kInv;
+              nd_2 = f2(nd * kInv, nd * kInv);
+              if (g == 0 && row < it->valid) {
+                const uint4 e = ext_columns<BF16>(0.f, nd);
+                *reinterpret_cast<uint2*>(&p.xstats[it->out_row + row].z) = make_uint2(e.z, e.w);
+              }
+            }
+            if (i < pre) {
+              arrive(bar->ds_full);
+              ph ^= 1u;
+              return true;
+            }
+          }
+        }
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
@@ -878,8 +943,15 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         ph ^= 1u;
         return true;
       };
-      if (n > 0 && tile(std::true_type(), 0))
-        for (int i = 1; i < n && tile(std::false_type(), i); ++i) {}
+      using Yes = std::true_type;
+      using No = std::false_type;
+      if (!KV && n > 0 && (pre > 0 || n == 1)) {
+        flush();
+        if constexpr (!KV)
+          for (int i = 0; i < n && tile(No(), Yes(), i); ++i) {}
+      } else if (n > 0 && tile(Yes(), No(), 0)) {
+        for (int i = 1; i < n && tile(No(), No(), i); ++i) {}
+      }
       if (failed) break;
       // dP of the last tile was the last MMA to read the stationary tiles (and
       // came after the last S), so the next item's can move in: its first
@@ -889,7 +961,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int next_n = next ? next->heads * next->nt0 + next->nt1 : 0;
       if (C::ATM && next_n > 0 && !copy_a()) break;
       const int valid = it->valid, limit = it->limit;
-      if (part * COLS < C::DV && row < limit) {
+      if (part * COLS < C::DV && row < limit && (KV || p.dq != nullptr)) {
         T* base = reinterpret_cast<T*>(!KV ? p.dq : is_dv ? (it->a_map ? p.dvc : p.dv) : (it->a_map ? p.dkc : p.dk));
         res_dst = base + (it->out_row + row) * (long long)D + it->dh * C::DV + part * COLS;
       }

@@ -42,7 +42,8 @@ def assert_within(got, val, bnd, what):
                              f"{got.flatten()[i]:.6g}, want {val.flatten()[i]:.6g} within {bnd.flatten()[i]:.3g}")
 
 
-def check(layout, dtype, B, H, HK, N, D, lens, ctx=None, causal=False, scale=None, seed=0, poison=True):
+def check(layout, dtype, B, H, HK, N, D, lens, ctx=None, causal=False, scale=None, seed=0, poison=True,
+          exact_delta=False):
     g = torch.Generator().manual_seed(seed)
     scale = D ** -0.5 if scale is None else scale
     q, do = rand(g, (B, H, N, D), dtype), rand(g, (B, H, N, D), dtype)
@@ -51,7 +52,7 @@ def check(layout, dtype, B, H, HK, N, D, lens, ctx=None, causal=False, scale=Non
     if ctx is not None:
         kc, vc = rand(g, (HK, sum(ctx), D), dtype), rand(g, (HK, sum(ctx), D), dtype)
         cmeta = meta_of(ctx, max(ctx))
-    val, bnd = batch_reference(q, k, v, do, scale, lens, kc, vc, ctx, causal)
+    val, bnd = batch_reference(q, k, v, do, scale, lens, kc, vc, ctx, causal, exact_delta)
     if layout == "dense":
         meta = None
         ins = [q, k, v, do]
@@ -130,6 +131,17 @@ def test_many_items():
     lens = [int(x) for x in torch.randint(0, 300, (70,), generator=g)]
     check("packed", BF16, 70, 8, 4, 300, 64, lens)
     check("padded", F16, 70, 8, 8, 300, 128, lens)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+@pytest.mark.parametrize("lens,ctx,causal", [([2, 3, 1, 20, 2], None, False), ([2, 3, 1, 20, 2], [5, 1, 0, 40, 3], False),
+                                             ([4, 1, 0, 7, 9], [13], True), ([64, 50, 2, 2, 2], None, False)])
+def test_few_keys(dtype, D, lens, ctx, causal):
+    """Rows of few keys: delta is summed in 32 bits, so its part of the bounds falls away."""
+    check("packed", dtype, 5, 4, 2, 64, D, lens, ctx=ctx, causal=causal, exact_delta=True)
+    if ctx is None:
+        check("padded", dtype, 5, 4, 2, 64, D, lens, exact_delta=True)
 
 
 def test_long():

@@ -29,8 +29,9 @@ def tiny(dtype):
     return 2.0 ** -25 if dtype == torch.float16 else 0.0
 
 
-def attention_with_gradients(q, k, v, do, scale, dtype):
-    """q, do [n, D], k, v [m, D] (float64) -> (values, bounds): dicts of o, lse, dq, dk, dv."""
+def attention_with_gradients(q, k, v, do, scale, dtype, exact_delta=False):
+    """q, do [n, D], k, v [m, D] (float64) -> (values, bounds): dicts of o, lse, dq, dk, dv.
+    ``exact_delta``: delta is summed from P dP in 32 bits (rows of few keys), E = 0."""
     u, t = unit(dtype), tiny(dtype)
     s = scale * (q @ k.T)
     lse = torch.logsumexp(s, 1)
@@ -39,7 +40,7 @@ def attention_with_gradients(q, k, v, do, scale, dtype):
     dp = do @ v.T
     ds = p * (dp - (do * o).sum(1, keepdim=True))
     pv = p @ v.abs()
-    err_delta = (do.abs() * ((2 * u + R32) * pv)).sum(1, keepdim=True)
+    err_delta = (do.abs() * ((2 * u + R32) * pv)).sum(1, keepdim=True) * (0.0 if exact_delta else 1.0)
     e_ds = u * ds.abs() + p * err_delta + R32 * (ds.abs() + p * (do.abs() @ v.abs().T)) + t
     a = abs(scale)
     val = dict(o=o, lse=lse, dq=scale * ds @ k, dk=scale * ds.T @ q, dv=p.T @ do)
@@ -49,7 +50,8 @@ def attention_with_gradients(q, k, v, do, scale, dtype):
     return val, bnd
 
 
-def batch_reference(q, k, v, do, scale, lens, kc=None, vc=None, ctx_lens=None, causal=False):
+def batch_reference(q, k, v, do, scale, lens, kc=None, vc=None, ctx_lens=None, causal=False,
+                    exact_delta=False):
     """Padded [B, H, N, D] inputs (context [HK, Tc, D]) -> (values, bounds) shaped like
     out (o), lse, dq, dk, dv, dkc, dvc; a shared head's or context's gradients are summed."""
     dtype, (B, H, N, D), HK = q.dtype, q.shape, k.shape[1]
@@ -80,7 +82,8 @@ def batch_reference(q, k, v, do, scale, lens, kc=None, vc=None, ctx_lens=None, c
                 ks.append(f[1][b2, hk, :lens[b2]])
                 vs.append(f[2][b2, hk, :lens[b2]])
                 parts.append(("m", (b2, hk, slice(0, lens[b2])), lens[b2]))
-            w, e = attention_with_gradients(f[0][b, h, :n], torch.cat(ks), torch.cat(vs), f[3][b, h, :n], scale, dtype)
+            w, e = attention_with_gradients(f[0][b, h, :n], torch.cat(ks), torch.cat(vs), f[3][b, h, :n], scale, dtype,
+                                            exact_delta)
             for dst, src in ((val, w), (bnd, e)):
                 dst["o"][b, h, :n] = src["o"]
                 dst["lse"][b, h, :n] = src["lse"]
