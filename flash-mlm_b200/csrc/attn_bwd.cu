@@ -157,6 +157,11 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
     return set_error(FMLM_ERR_INVALID, "out and lse are required; out and dout must be 16-byte aligned");
   if (!aligned32(a->dq) || !aligned32(a->dk) || !aligned32(a->dv))
     return set_error(FMLM_ERR_INVALID, "dq, dk, dv must be 32-byte aligned");
+  // float16: lse in units of the scores has to fit three float16 numbers
+  const bool bf16 = a->dtype == FMLM_DTYPE_BF16;
+  const float mag = std::fabs(a->scale);
+  if (!(mag <= (bf16 ? 0x1p64f : 0x1p20f)) || (!bf16 && mag < 0x1p-24f))
+    return set_error(FMLM_ERR_INVALID, "scale must be finite, at most 2^64 in magnitude, for float16 in [2^-24, 2^20]");
   const int64_t rows = qb * a->num_heads * qr;
   if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < fmlm_attn_bwd_workspace_bytes(rows))
     return set_error(FMLM_ERR_INVALID, "workspace too small (%zu bytes needed)", fmlm_attn_bwd_workspace_bytes(rows));
@@ -188,22 +193,20 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.dvc = a->dv_context;
   p.scale = a->scale;
   // The exponent's scale, kept away from 0: the KV pass divides lse by it.  At
-  // 2^-24 scores of any size that float16 or bfloat16 attention meets (below a
-  // thousand) move the exponent by less than 2^-14.
+  // 2^-100 no bfloat16 score moves the exponent; float16's range ends earlier,
+  // and its scales are refused above instead.
   const float sl2 = a->scale * 1.4426950408889634f;
-  p.scale_log2 = std::fabs(sl2) < 0x1p-24f ? (sl2 < 0.f ? -0x1p-24f : 0x1p-24f) : sl2;
+  p.scale_log2 = std::fabs(sl2) < 0x1p-100f ? 0x1p-100f : sl2;
   // A power of two near 1 / scale_log2 (float16 holds 2^-14 .. 2^15), so that
   // what the 16-bit columns hold is of lse's own magnitude.
-  const int e = std::min(15, std::max(-14, -std::ilogb(p.scale_log2)));
+  const int e = std::min(bf16 ? 100 : 15, std::max(bf16 ? -100 : -14, -std::ilogb(p.scale_log2)));
   p.ext_unit = std::ldexp(1.f, e);
   const float ext_mul = 1.f / (p.scale_log2 * p.ext_unit);
   // -400 in the exponent; one 16-bit number is near enough
   const float none = -400.f * ext_mul;
-  p.xnone = make_uint4(a->dtype == FMLM_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(none))
-                                                   : __half_as_ushort(__float2half_rn(none)), 0, 0, 0);
+  p.xnone = make_uint4(bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(none)) : __half_as_ushort(__float2half_rn(none)), 0, 0, 0);
   p.err = a->error_word;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == FMLM_DTYPE_BF16 ? dispatch_bwd<true>(a, p, ext_mul, rows, s)
-                                     : dispatch_bwd<false>(a, p, ext_mul, rows, s);
+  return bf16 ? dispatch_bwd<true>(a, p, ext_mul, rows, s) : dispatch_bwd<false>(a, p, ext_mul, rows, s);
 }

@@ -55,7 +55,7 @@ def _view(x: torch.Tensor) -> _lib.View4:
     return _lib.View4(x.data_ptr(), t, h, 1, st, sh, h * t * d)
 
 
-def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
+def _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal):
     """Shapes, types and devices of a training call; returns the layout code."""
     if q.ndim not in (3, 4) or k.ndim != q.ndim or v.ndim != q.ndim:
         raise ValueError("q/k/v must be rank-4 tensors [B, H, N, D] or packed rank-3 tensors [H, T, D]")
@@ -68,7 +68,10 @@ def _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal):
     if hk < 1 or h < 1 or h % hk != 0:
         raise ValueError("the heads of q must be a multiple of the heads of k and v")
     validate_head_dim_supported(qs[-1])
-    _lib.dtype_code(q.dtype)
+    half = _lib.dtype_code(q.dtype) == _lib.FMLM_DTYPE_F16
+    # float16: the backward pass holds lse / scale in three float16 numbers
+    if not abs(scale) <= (2.0**20 if half else 2.0**64) or (half and abs(scale) < 2.0**-24):
+        raise ValueError("scale must be finite, at most 2^64 in magnitude, for float16 in [2^-24, 2^20]")
     packed = q.ndim == 3
     if packed:
         if q_meta is None:
@@ -141,7 +144,7 @@ def flash_attn_mlm_fwd(
     and lse (float32, q's shape without D): the natural log of each row's
     softmax denominator, undefined at padding rows.
     """
-    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    layout = _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     _require_packed(q, context_k, causal_query_seq_attn)
     return _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
 
@@ -215,7 +218,7 @@ def flash_attn_mlm_bwd(
     What is not needed (``need_dq``, ``need_dkv``), and the context's without
     a context, is None.
     """
-    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    layout = _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     _require_packed(q, context_k, causal_query_seq_attn)
     for name, x in (("dout", dout), ("out", out)):
         if x.shape != q.shape or x.dtype != q.dtype or x.device != q.device:
@@ -350,7 +353,7 @@ def flash_attn_mlm_train(
     To capture the backward pass into a CUDA graph, call ``flash_attn_mlm_fwd``
     and ``flash_attn_mlm_bwd``, which involve no autograd graph.
     """
-    layout = _validate(q, k, v, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
+    layout = _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     if q.ndim == 4 and (context_k is not None or causal_query_seq_attn):
         qp, kp, vp = (_Pack.apply(x, q_meta) for x in (q, k, v))
         out = _Attention.apply(qp, kp, vp, context_k, context_v, _lib.FMLM_BWD_PACKED, scale, q_meta, context_meta,

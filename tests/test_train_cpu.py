@@ -129,3 +129,22 @@ def test_c_refuses_head_dim_and_null():
         v.row_stride, v.head_stride = 48, 480
         setattr(a, f, v)
     assert L.fmlm_attn_bwd(ctypes.byref(a), None) == -2
+
+
+@pytest.mark.parametrize("entry", ["fwd", "bwd", "train"])
+@pytest.mark.parametrize("dtype,scale", [(F16, 0.0), (F16, 2.0**-25), (F16, -(2.0**21)), (F16, float("nan")),
+                                         (torch.bfloat16, float("inf")), (torch.bfloat16, 2.0**65)])
+def test_scale_refusals(entry, dtype, scale):
+    x = z(2, 4, 8, 64, dtype=dtype)
+    kw = dict(q=x, k=x, v=x, scale=scale)
+    if entry == "bwd":
+        kw.update(dout=x, out=x, lse=torch.zeros(2, 4, 8))
+    with pytest.raises(ValueError, match="scale"):
+        getattr(flash_mlm, f"flash_attn_mlm_{entry}")(**kw)
+
+
+@pytest.mark.parametrize("dtype,scale", [(0, 0.0), (0, 2.0**21), (1, float("nan")), (1, 2.0**65)])
+def test_c_scale_refusals(dtype, scale):
+    L = _lib.lib()
+    assert L.fmlm_attn_bwd(ctypes.byref(bwd_args(dtype=dtype, scale=scale)), None) == -1
+    assert "scale" in L.fmlm_last_error().decode()
