@@ -491,8 +491,9 @@ __global__ void __launch_bounds__(AttnCfg<D, NQ>::THREADS) __maxnreg__((AttnCfg<
     // tile (K for MLA) hold the caller's padding, which may be non-finite; P is
     // zero there but 0 * NaN is not, so they are cleared once the tile lands.
     // For a V tile the clearing is deferred to just before the producer's next
-    // wait for a free K/V stage (the only wait that can depend on V), so the
-    // next item's Q and first blocks are requested without waiting for it.
+    // wait for a free K/V stage (before an item without keys is passed, the
+    // only wait that can depend on V), so the next item's Q and first blocks
+    // are requested without waiting for it.
     uint8_t* pend_tile = nullptr;
     int pend_valid = 0;
     uint64_t* pend_bar = nullptr;
@@ -566,6 +567,10 @@ __global__ void __launch_bounds__(AttnCfg<D, NQ>::THREADS) __maxnreg__((AttnCfg<
       const uint32_t qn_par = (((ring + 1) / C::QBUF) & 1u) ^ 1u;
       const Item itn = (next < num_items) ? decode_item<C::PAIR, BN, C::NDH>(p, next) : it;
       const int nb = it.nblocks();
+      // An item without keys (an empty sequence of a padded output) waits for no
+      // stage, and its Q buffer is released when the MMA warps reach it, which
+      // takes the previous item's V.
+      if (nb == 0) resolve_fix();
       if constexpr (C::SPLIT_KV) {
         // K(j) is requested when its stage's previous K has been read by S;
         // V(j) one block later, when its stage's previous V has been read by
