@@ -31,6 +31,14 @@
 // ranges, which it then walks twice) sums delta = sum_k P dP itself, in 32 bits
 // (1.4), and leaves it for the KV pass, which runs after.
 //
+// P and dS are rounded to 16 bits for the tensor cores, half a step of each
+// term: next to the rounding of the result that is a factor of 1.4 in a
+// gradient's error when many terms average it, and up to 2 when there are few.
+// So items that stream few rows, or hold the few rows of a short sequence, give
+// P and dS as the sum of two 16-bit numbers, the second in the TMEM columns
+// that the first leaves free, for another K walk of the accumulating MMAs
+// (factor 1.0; all items that way would add 2 to the 7 matrix products).
+//
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
 // warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs,
@@ -112,6 +120,7 @@ struct BwdCfg {
   static constexpr int SMEM_TILES = 2 * A_BYTES + 2 * STAGES * B_BYTES + AX_BYTES + 2 * STAGES * BX_BYTES;
   static constexpr int SUM_BYTES = KV ? 0 : 2 * EW_GROUPS * BM * 4;  // Q: delta's partial sums, twice
   static constexpr int EXACT_KEYS = 64;  // Q: items of several tiles with at most so many keys sum delta themselves
+  static constexpr int FEW_TERMS = 128, FEW_ROWS = 8;  // items whose P and dS keep a second part (see above)
   static constexpr int RING = 4;
   static constexpr int ITEM_BYTES = 96;
   static constexpr int SMEM_BYTES = SMEM_TILES + 512 + RING * ITEM_BYTES + SUM_BYTES + 1024;
@@ -128,6 +137,7 @@ struct BwdItem {
   int row1, end1, nt1;         // second range (main)
   int stat_h;                  // KV: stats rows of one streamed head
   int pre;                     // Q: tiles walked first for delta alone (0 or all of them)
+  int few;                     // few terms or few rows: P and dS keep a second 16-bit part
   long long out_row;           // output row of the tile's row 0 (also its stats row in the Q pass)
   long long stat0;             // KV: stats row of (head h0, streamed row 0)
 };
@@ -179,10 +189,11 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   it.h0 = C::KV ? h * p.G : h / p.G;
   it.stat_h = 0;
   it.stat0 = 0;
+  int tile = 0;  // of its sequence
   if (ctx) {
     const int c = find_slot_owner(p.cu_c, p.C, v, lane);
     const int c0 = min(max(__ldg(p.cu_c + c), 0), p.Tc), c1 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
-    const int t = v - ((c0 >> 7) + c);
+    const int t = tile = v - ((c0 >> 7) + c);
     it.a_row = c0 + t * 128;
     it.valid = it.limit = min(max(c1 - it.a_row, 0), t >= 0 ? 128 : 0);
     it.out_row = (long long)h * p.Tc + it.a_row;
@@ -193,7 +204,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   } else if (packed) {
     const int b = find_slot_owner(p.cu_q, p.B, v, lane);
     const int s0 = min(max(__ldg(p.cu_q + b), 0), p.T), s1 = min(max(__ldg(p.cu_q + b + 1), 0), p.T);
-    const int t = v - ((s0 >> 7) + b);
+    const int t = tile = v - ((s0 >> 7) + b);
     it.a_row = s0 + t * 128;
     it.valid = it.limit = min(max(s1 - it.a_row, 0), t >= 0 ? 128 : 0);
     it.out_row = (long long)h * p.T + it.a_row;
@@ -217,6 +228,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
     const int b = v / per_seq, t = v % per_seq;
     int L = p.N;
     if (p.layout == FMLM_BWD_PADDED) L = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
+    tile = t;
     it.a_row = t * 128;
     it.a_b = it.b = b;
     it.valid = min(max(L - it.a_row, 0), 128);
@@ -230,9 +242,11 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   it.nt0 = tiles(it.row0, it.end0);
   if (it.valid == 0) it.nt0 = it.nt1 = 0;
   it.pre = 0;
+  const int n = it.nt0 + it.nt1, terms = max(it.end0 - it.row0, 0) + max(it.end1 - it.row1, 0);
+  it.few = (it.valid <= C::FEW_ROWS && tile == 0) || (long long)it.heads * terms <= C::FEW_TERMS;
   if constexpr (!C::KV) {
-    const int n = it.nt0 + it.nt1, keys = max(it.end0 - it.row0, 0) + max(it.end1 - it.row1, 0);
-    if (n > 1 && keys <= C::EXACT_KEYS) it.pre = n;
+    if (n > 1 && terms <= C::EXACT_KEYS) it.pre = n;
+    if (n == 1 || it.pre > 0) it.few = 1;
     // dq not asked for: only items that have a delta to leave
     if (p.dq == nullptr && n != 1 && it.pre == 0) it.valid = it.limit = it.nt0 = it.nt1 = 0;
   }
@@ -350,6 +364,19 @@ __device__ __forceinline__ uint32_t pack2(F2 v) {
   float a, b;
   unf2(v, a, b);
   return pack2<BF16>(a, b);
+}
+
+template <bool BF16>
+__device__ __forceinline__ F2 unpack2(uint32_t u) {
+  if constexpr (BF16) return f2u(u << 16, u & 0xffff0000u);
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  return f2(v.x, v.y);
+}
+
+// What rounding v to the pair u left over, as another pair.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_rest(F2 v, uint32_t u) {
+  return pack2<BF16>(fma2(unpack2<BF16>(u), f2(-1.f, -1.f), v));
 }
 
 // 16-byte half h of row r of a tile of 32-byte rows in the 32-byte swizzle.
@@ -639,9 +666,10 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     };
     // accumulators: D[128, DV] += A[128, BN] (16-bit, TMEM) B[BN, DV], as A's
     // columns are handed over.  They are in EW_GROUPS pieces, `piece` TMEM
-    // columns apart; a half is every other K step.
-    auto issue_acc = [&](uint64_t* full, uint32_t ph, uint32_t d, uint32_t a_tm, uint32_t piece, uint32_t b_base, bool acc,
-                         uint64_t* done) -> bool {
+    // columns apart; a half is every other K step.  `rest` (0: none): A's second
+    // part, in pieces NC columns apart.
+    auto issue_acc = [&](uint64_t* full, uint32_t ph, uint32_t d, uint32_t a_tm, uint32_t piece, uint32_t rest,
+                         uint32_t b_base, bool acc, uint64_t* done) -> bool {
       constexpr int KP = C::NC / 16;  // K steps per piece
       constexpr int STEP = C::SPLIT ? KP : 1;
       const uint32_t b = (b_base >> 4) | lbo_mn;
@@ -654,7 +682,14 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           for (int kk = half; kk < BN / 16; kk += STEP)
             mma_ts(d, a_tm + (kk / KP) * piece + (kk % KP) * 8, b + (kk * 16 * SWB >> 4), hi, idesc_acc,
                    kk > 0 ? 1u : acc ? 1u : 0u);
-          if (half == STEP - 1) umma_commit(done);
+          if (half == STEP - 1) {
+            if (rest != 0) {
+#pragma unroll 1
+              for (int kk = 0; kk < BN / 16; ++kk)
+                mma_ts(d, rest + (kk / KP) * C::NC + (kk % KP) * 8, b + (kk * 16 * SWB >> 4), hi, idesc_acc, 1u);
+            }
+            umma_commit(done);
+          }
         }
       }
       return true;
@@ -695,6 +730,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       // valid rows of each range's last tile
       const int last0 = slot->end0 - slot->row0 - (nt0 - 1) * BN, last1 = slot->end1 - slot->row1 - (nt1 - 1) * BN;
       const uint32_t dh_off = (slot->dh * C::DV / C::SLAB_COLS) * (BN * SWB);
+      const bool few = slot->few != 0;
+      const uint32_t rest_p = few ? tmem_base + C::TM_S + C::NC / 2 : 0, rest_ds = few ? tmem_base + C::TM_DP + C::NC / 2 : 0;
       release_item(ring);
       if (n == 0) continue;
       if (!wait(C::ATM ? &bar->a_tm : &bar->a_full, aload & 1u)) break;
@@ -743,25 +780,27 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         // The next S as soon as its columns are free: this S is in registers,
         // and (KV, P over S) P is consumed, the MMAs running in order.  One
         // stage only: its tile B1 takes the place of the one dS still needs.
+        // P's second part is over S (a separate P's too), so that S waits as well.
         constexpr bool kEarlyS = C::SEP_P || !KV;
+        const bool early = kEarlyS && !(KV && few);
         if (kEarlyS && STAGES > 1) {
-          if (!wait(&bar->s_free, ph) || (more && !do_s())) { ok = false; break; }
+          if (!wait(&bar->s_free, ph) || (early && more && !do_s())) { ok = false; break; }
         }
         if (first) {
           if (!wait(&bar->acc_empty, acc_ph)) { ok = false; break; }
           acc_ph ^= 1u;
         }
         if constexpr (KV) {
-          if (!issue_acc(bar->p_full, ph, tmem_base + C::TM_ACC1, tmem_base + C::TM_P, C::SEP_P ? C::NC / 2 : C::NC, b2,
-                         !first, &bar->b2_empty[c_st.i])) { ok = false; break; }
+          if (!issue_acc(bar->p_full, ph, tmem_base + C::TM_ACC1, tmem_base + C::TM_P, C::SEP_P ? C::NC / 2 : C::NC,
+                         rest_p, b2, !first, &bar->b2_empty[c_st.i])) { ok = false; break; }
           if (C::SEP_P) commit(&bar->p_free);
         }
-        if (!kEarlyS && STAGES > 1 && more && !do_s()) { ok = false; break; }
+        if (!early && STAGES > 1 && more && !do_s()) { ok = false; break; }
         if (!KV && left > n - pre) {  // delta only: dP is read, B1 is free
           if (!wait(bar->ds_full, ph)) { ok = false; break; }
           commit(&bar->b1_empty[c_st.i]);
-        } else if (!issue_acc(bar->ds_full, ph, tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, b1, !first,
-                              &bar->b1_empty[c_st.i])) {
+        } else if (!issue_acc(bar->ds_full, ph, tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, rest_ds, b1,
+                              !first, &bar->b1_empty[c_st.i])) {
           ok = false;
           break;
         }
@@ -794,11 +833,14 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     auto ld = [&](uint32_t a, uint32_t(&r)[NC]) {
       if constexpr (NC == 32) tmem_ld_x32(a, r); else tmem_ld_x16(a, r);
     };
-    // Stores packed pairs and hands them over, half h of them with SPLIT.
-    auto give = [&](uint32_t a, const uint32_t(&r)[NC / 2], int h, uint64_t* full) {
+    // Stores packed pairs, half h of them with SPLIT; give hands them over.
+    auto put = [&](uint32_t a, const uint32_t(&r)[NC / 2], int h) {
       if constexpr (C::SPLIT) tmem_st_x8_nowait(a + h * 8, r + h * 8);
       else if constexpr (NC == 32) tmem_st_x16_nowait(a, r);
       else tmem_st_x8_nowait(a, r);
+    };
+    auto give = [&](uint32_t a, const uint32_t(&r)[NC / 2], int h, uint64_t* full) {
+      put(a, r, h);
       tmem_wait_st();
       arrive(full + h);
     };
@@ -856,8 +898,9 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const F2 nl_2 = f2(rs.x, rs.x);
       F2 nd_2 = f2(rs.y * kInv, rs.y * kInv);
       // (The first tile apart, so that the waiting results leave their registers
-      // there; and apart the items that sum delta themselves.)
-      auto tile = [&](auto first, auto exact, int i) -> bool {
+      // there; and apart the items of few terms, of which some sum delta themselves.)
+      auto tile = [&](auto first, auto few, int i) -> bool {
+        constexpr bool kFew = decltype(few)::value;
         if (!wait(&bar->s_full, ph)) return false;
         tc_fence_after();
         uint32_t x[NC];
@@ -865,7 +908,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         ld(tS, x);
         if (C::SEP_P || !KV) arrive(&bar->s_free);
         if constexpr (kDefer && decltype(first)::value) flush();
-        uint32_t pk[NC / 2];
+        uint32_t pk[NC / 2], pk2[NC / 2];  // (pk2: few only)
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
@@ -877,16 +920,20 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
           }
           if constexpr (KV) {
 #pragma unroll
-            for (int c = h * HC; c < (h + 1) * HC; ++c) pk[c] = pack2<BF16>(pr[c]);
+            for (int c = h * HC; c < (h + 1) * HC; ++c) {
+              pk[c] = pack2<BF16>(pr[c]);
+              if constexpr (kFew) pk2[c] = pack_rest<BF16>(pr[c], pk[c]);
+            }
             if (C::SEP_P) {
               if (!wait(&bar->p_free, ph ^ 1u)) return false;
               tc_fence_after();
             }
+            if constexpr (kFew) put(tS + NC / 2, pk2, h);
             give(tP, pk, h, bar->p_full);
           }
         }
         if constexpr (!KV) {
-          const int j = decltype(exact)::value && i >= pre ? i - pre : i;
+          const int j = kFew && i >= pre ? i - pre : i;
           const int valid = (j >= nt0 ? it->end1 - (it->row1 + (j - nt0) * BN) : it->end0 - (it->row0 + j * BN)) - g * NC;
           if (valid < NC) {
 #pragma unroll
@@ -900,7 +947,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         if (!wait(&bar->dp_full, ph)) return false;
         tc_fence_after();
         ld(tDP, x);
-        if constexpr (!KV && decltype(exact)::value) {
+        if constexpr (!KV && kFew) {
           if (i < pre || n == 1) {
             F2 acc = f2(0.f, 0.f);
 #pragma unroll
@@ -936,8 +983,11 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             F2 d = f2u(x[2 * c], x[2 * c + 1]);
             if constexpr (!KV) d = fma2(d, kinv_2, nd_2);
             else if constexpr (!BF16) d = mul2(d, kinv_2);
-            pk[c] = pack2<BF16>(mul2(pr[c], d));
+            d = mul2(pr[c], d);
+            pk[c] = pack2<BF16>(d);
+            if constexpr (kFew) pk2[c] = pack_rest<BF16>(d, pk[c]);
           }
+          if constexpr (kFew) put(tDP + NC / 2, pk2, h);
           give(tDP, pk, h, bar->ds_full);
         }
         ph ^= 1u;
@@ -945,10 +995,9 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       };
       using Yes = std::true_type;
       using No = std::false_type;
-      if (!KV && n > 0 && (pre > 0 || n == 1)) {
+      if (n > 0 && it->few) {
         flush();
-        if constexpr (!KV)
-          for (int i = 0; i < n && tile(No(), Yes(), i); ++i) {}
+        for (int i = 0; i < n && tile(No(), Yes(), i); ++i) {}
       } else if (n > 0 && tile(Yes(), No(), 0)) {
         for (int i = 1; i < n && tile(No(), No(), i); ++i) {}
       }

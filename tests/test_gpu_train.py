@@ -43,7 +43,7 @@ def assert_within(got, val, bnd, what):
 
 
 def check(layout, dtype, B, H, HK, N, D, lens, ctx=None, causal=False, scale=None, seed=0, poison=True,
-          exact_delta=False):
+          exact_delta=False, two_parts=False):
     g = torch.Generator().manual_seed(seed)
     scale = D ** -0.5 if scale is None else scale
     q, do = rand(g, (B, H, N, D), dtype), rand(g, (B, H, N, D), dtype)
@@ -52,7 +52,7 @@ def check(layout, dtype, B, H, HK, N, D, lens, ctx=None, causal=False, scale=Non
     if ctx is not None:
         kc, vc = rand(g, (HK, sum(ctx), D), dtype), rand(g, (HK, sum(ctx), D), dtype)
         cmeta = meta_of(ctx, max(ctx))
-    val, bnd = batch_reference(q, k, v, do, scale, lens, kc, vc, ctx, causal, exact_delta)
+    val, bnd = batch_reference(q, k, v, do, scale, lens, kc, vc, ctx, causal, exact_delta, two_parts)
     if layout == "dense":
         meta = None
         ins = [q, k, v, do]

@@ -134,3 +134,30 @@ def test_many_short_contexts():
     assert torch.equal(out[:, a:], out1) and torch.equal(lse[:, a:], lse1)
     for i, (x, y) in enumerate(zip(grads, grads1)):
         assert torch.equal(x[:, (a if i < 3 else b):], y), i
+
+
+FEW = [("packed", [2, 3, 1, 20, 2], None, False, 2), ("packed", [2, 3, 1, 20, 2], [5, 1, 0, 40, 3], False, 2),
+       ("packed", [4, 1, 0, 7, 9], [13], True, 2), ("packed", [64, 50, 2, 2, 2], None, False, 2),
+       ("padded", [64, 30, 0, 1, 7], None, False, 2), ("dense", [64] * 5, None, False, 2), ("dense", [16] * 2, None, False, 1)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout,lens,ctx,causal,HK", FEW)
+def test_gradients_of_few_terms(dtype, D, layout, lens, ctx, causal, HK):
+    """At most 128 streamed rows to every tile (64 keys; two query heads of 64): P and dS in two 16-bit numbers."""
+    N = max(lens) if layout == "dense" else 64
+    check(layout, dtype, len(lens), 4 if HK == 2 else 8, HK, N, D, lens, ctx=ctx, causal=causal, exact_delta=True,
+          two_parts=True)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_items_of_few_and_of_many_terms_in_turn(dtype, D):
+    """Lengths on both sides of the limits, several items per block: the two forms after one another."""
+    g = torch.Generator().manual_seed(9)
+    lens = [int(x) for x in torch.randint(0, 3, (60,), generator=g)] + [600, 8, 9, 129, 64, 65, 300] * 3
+    order = torch.randperm(len(lens), generator=g).tolist()
+    lens = [lens[i] for i in order]
+    check("packed", dtype, len(lens), 6, 3, 600, D, lens)
+    check("packed", dtype, len(lens), 2, 1, 600, D, lens, ctx=[3])

@@ -13,6 +13,8 @@ head_dim and over keys):
       |err| <= e_dS = u |dS| + P E + r (|dS| + P |dO||v|^T) + t
   where t is float16's smallest half step (2^-25), 0 for bfloat16
 * dQ = scale dS k:  |err| <= scale e_dS |k| + u |dQ|;  dK alike with e_dS^T |q|
+* where P and dS are the sum of two 16-bit numbers, u^2 stands for the u of their
+  rounding (the second number is rounded, to u of at most u of the whole);
 * every float16 output may also lose t to its own subnormals.
 """
 
@@ -29,10 +31,11 @@ def tiny(dtype):
     return 2.0 ** -25 if dtype == torch.float16 else 0.0
 
 
-def attention_with_gradients(q, k, v, do, scale, dtype, exact_delta=False):
+def attention_with_gradients(q, k, v, do, scale, dtype, exact_delta=False, two_parts=False):
     """q, do [n, D], k, v [m, D] (float64) -> (values, bounds): dicts of o, lse, dq, dk, dv.
-    ``exact_delta``: delta is summed from P dP in 32 bits (rows of few keys), E = 0."""
+    ``exact_delta``: delta is summed from P dP in 32 bits (rows of few keys), E = 0.  ``two_parts``: P and dS in two 16-bit numbers (gradients of few terms)."""
     u, t = unit(dtype), tiny(dtype)
+    up = u * u if two_parts else u
     s = scale * (q @ k.T)
     lse = torch.logsumexp(s, 1)
     p = torch.exp(s - lse[:, None])
@@ -41,17 +44,17 @@ def attention_with_gradients(q, k, v, do, scale, dtype, exact_delta=False):
     ds = p * (dp - (do * o).sum(1, keepdim=True))
     pv = p @ v.abs()
     err_delta = (do.abs() * ((2 * u + R32) * pv)).sum(1, keepdim=True) * (0.0 if exact_delta else 1.0)
-    e_ds = u * ds.abs() + p * err_delta + R32 * (ds.abs() + p * (do.abs() @ v.abs().T)) + t
+    e_ds = up * ds.abs() + p * err_delta + R32 * (ds.abs() + p * (do.abs() @ v.abs().T)) + t
     a = abs(scale)
     val = dict(o=o, lse=lse, dq=scale * ds @ k, dk=scale * ds.T @ q, dv=p.T @ do)
     bnd = dict(o=(u + R32) * pv + u * o.abs() + t, lse=R32 * (1 + lse.abs()),
                dq=a * e_ds @ k.abs() + u * val["dq"].abs() + t, dk=a * e_ds.T @ q.abs() + u * val["dk"].abs() + t,
-               dv=(u + R32) * p.T @ do.abs() + u * val["dv"].abs() + t)
+               dv=(up + R32) * p.T @ do.abs() + u * val["dv"].abs() + t)
     return val, bnd
 
 
 def batch_reference(q, k, v, do, scale, lens, kc=None, vc=None, ctx_lens=None, causal=False,
-                    exact_delta=False):
+                    exact_delta=False, two_parts=False):
     """Padded [B, H, N, D] inputs (context [HK, Tc, D]) -> (values, bounds) shaped like
     out (o), lse, dq, dk, dv, dkc, dvc; a shared head's or context's gradients are summed."""
     dtype, (B, H, N, D), HK = q.dtype, q.shape, k.shape[1]
@@ -83,7 +86,7 @@ def batch_reference(q, k, v, do, scale, lens, kc=None, vc=None, ctx_lens=None, c
                 vs.append(f[2][b2, hk, :lens[b2]])
                 parts.append(("m", (b2, hk, slice(0, lens[b2])), lens[b2]))
             w, e = attention_with_gradients(f[0][b, h, :n], torch.cat(ks), torch.cat(vs), f[3][b, h, :n], scale, dtype,
-                                            exact_delta)
+                                            exact_delta, two_parts)
             for dst, src in ((val, w), (bnd, e)):
                 dst["o"][b, h, :n] = src["o"]
                 dst["lse"][b, h, :n] = src["lse"]
