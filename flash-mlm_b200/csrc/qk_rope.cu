@@ -16,9 +16,9 @@
 // What keeps memory busy is the loads that each thread has under way: four
 // heads at a time forward, two backward, and the registers for them rather than
 // more warps.  16 x 4096 tokens, 32 + 8 heads of 128, a projection's strides:
-// forward 227 us (5.9 TB/s; with registers capped for two blocks per SM 254,
-// two heads at a time 268, eight 282), backward 400 us (5.0 TB/s; one head at a
-// time and three blocks 445, weights in registers 439).
+// forward 222 us (6.0 TB/s; with registers capped for two blocks per SM 254,
+// two heads at a time 268, eight 282), backward 388 us (5.2 TB/s; weights in
+// registers 421, one head at a time and three blocks 445).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -172,7 +172,7 @@ typedef struct fmlm_attn_bwd_args {
   int32_t seq_len;                  /* N (dense, padded) */
   int32_t causal_query_seq_attn;    /* packed only */
   int32_t context_entries;          /* 0: no context; 1: one shared by all sequences; batch: one each (packed only) */
-  float scale;
+  float scale;                      /* finite, at most 2^64 in magnitude; float16: 2^-24 to 2^20 */
   int64_t total_q_len;              /* packed: T */
   int64_t total_context_len;        /* rows per head of the context */
   fmlm_view4 q, k, v, dout;         /* q, dout: num_heads heads; k, v: kv_heads */
