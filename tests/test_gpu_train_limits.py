@@ -161,3 +161,22 @@ def test_items_of_few_and_of_many_terms_in_turn(dtype, D):
     lens = [lens[i] for i in order]
     check("packed", dtype, len(lens), 6, 3, 600, D, lens)
     check("packed", dtype, len(lens), 2, 1, 600, D, lens, ctx=[3])
+
+
+@pytest.mark.parametrize("how", ["projection", "window", "unaligned"])
+def test_padded_with_context_in_other_strides(how):
+    """The layout that is packed on the way: q, k, v and the context as a program may hold them,
+    and the gradient of a sum (one element, expanded)."""
+    from test_gpu_train_use import relaid
+
+    g = torch.Generator().manual_seed(4)
+    lens, ctx = [70, 0, 33, 129], [20, 5, 0, 140]
+    q, k, v = (rand(g, (4, h, 129, 64), BF16) for h in (4, 2, 2))
+    kc, vc = (rand(g, (2, sum(ctx), 64), BF16) for _ in range(2))
+    results = []
+    for f in (lambda x: x, lambda x: relaid(x, how)):
+        leaves = [f(x).detach().requires_grad_() for x in (q, k, v, kc, vc)]
+        out = fm().flash_attn_mlm_train(*leaves[:3], 0.125, meta_of(lens, 129), *leaves[3:], meta_of(ctx, 140), True)
+        results.append([out.detach(), *torch.autograd.grad(out.sum(), leaves)])
+    no_errors()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
