@@ -107,6 +107,11 @@ struct BwdCfg {
   // starts that much earlier (8192 tokens: KV pass 759 -> 726 us; the Q pass,
   // where only dP waits, gained nothing).
   static constexpr bool SPLIT = KV && D == 128;
+  // Two buffers of dP / dS (Q, where TMEM has the columns): the next dP is
+  // issued with the next S instead of behind this tile's accumulation (head_dim
+  // 64, a shared context of 1024 keys: Q pass 136 -> 130 us; with earlier
+  // sequences 425 -> 405).
+  static constexpr bool DB = !KV && D <= 64;
   static constexpr int EW_GROUPS = 4;
   static constexpr int EW_WARPS = 4 * EW_GROUPS;
   static constexpr int TMA_WARP = EW_WARPS;
@@ -115,7 +120,7 @@ struct BwdCfg {
   static constexpr int THREADS = 32 * (EW_WARPS + (KV ? 3 : 2));
   static constexpr int NC = BN / EW_GROUPS;  // score columns per element-wise warp
   static constexpr int TM_S = 0, TM_DP = BN, TM_P = SEP_P ? 2 * BN : 0;
-  static constexpr int TM_ACC1 = 2 * BN + (SEP_P ? BN / 2 : 0), TM_ACC2 = TM_ACC1 + (KV ? DV : 0);
+  static constexpr int TM_ACC1 = (DB ? 3 : 2) * BN + (SEP_P ? BN / 2 : 0), TM_ACC2 = TM_ACC1 + (KV ? DV : 0);
   static constexpr int TM_A1 = TM_ACC2 + DV, TM_A2 = TM_A1 + (ATM ? D / 2 : 0);
   static constexpr int TMEM_USED = TM_A2 + (ATM ? D / 2 : 0);
   static_assert(TMEM_USED <= 512, "TMEM budget");
@@ -263,9 +268,9 @@ struct __align__(8) BwdBarriers {
   uint64_t a_full, a_empty;
   uint64_t b1_full[4], b2_full[4], b1_empty[4], b2_empty[4];
   uint64_t a_tm;              // element-wise -> MMA: the stationary tiles are in TMEM
-  uint64_t s_full, dp_full;   // MMA -> element-wise: S / dP complete
+  uint64_t s_full, dp_full[2];  // MMA -> element-wise: S / dP (of either buffer) complete
   uint64_t s_free;            // element-wise -> MMA: S is in registers
-  uint64_t p_full[2], ds_full[2];  // element-wise -> MMA: P / dS written (or its first, second half)
+  uint64_t p_full[2], ds_full[2];  // element-wise -> MMA: P / dS written (its first, second half; or dS in either buffer)
   uint64_t p_free;            // MMA -> element-wise (separate P): P consumed
   uint64_t sum_full;          // Q: every warp's part of delta is in shared memory
   uint64_t acc_full, acc_empty;
@@ -449,11 +454,11 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       mbar_init(&bar->item_empty[i], C::EW_WARPS + (KV ? 2 : 1));
     }
     mbar_init(&bar->s_full, 1);
-    mbar_init(&bar->dp_full, 1);
     mbar_init(&bar->a_tm, C::EW_WARPS);
     mbar_init(&bar->s_free, C::EW_WARPS);
     mbar_init(&bar->p_free, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->dp_full[i], 1);
       mbar_init(&bar->p_full[i], C::EW_WARPS);
       mbar_init(&bar->ds_full[i], C::EW_WARPS);
     }
@@ -728,7 +733,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       }
     };
     Stage s_st, d_st, c_st;  // stages of the next S, the next dP, the current accumulations
-    uint32_t aload = 0, ph = 0, acc_ph = 1;
+    uint32_t aload = 0, ph = 0, ph2 = 0, acc_ph = 1;  // ph2: of a barrier that every other tile uses (DB)
     for (uint32_t ring = 0;; ++ring) {
       const BwdItem* slot = take_item(ring);
       if (!slot) break;
@@ -737,7 +742,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int last0 = slot->end0 - slot->row0 - (nt0 - 1) * BN, last1 = slot->end1 - slot->row1 - (nt1 - 1) * BN;
       const uint32_t dh_off = (slot->dh * C::DV / C::SLAB_COLS) * (BN * SWB);
       const bool few = slot->few != 0;
-      const uint32_t rest_p = few ? tmem_base + C::TM_S + C::NC / 2 : 0, rest_ds = few ? tmem_base + C::TM_DP + C::NC / 2 : 0;
+      const uint32_t rest_p = few ? tmem_base + C::TM_S + C::NC / 2 : 0;
       release_item(ring);
       if (n == 0) continue;
       if (!wait(C::ATM ? &bar->a_tm : &bar->a_full, aload & 1u)) break;
@@ -764,22 +769,24 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         s_st.next();
         return true;
       };
-      auto do_dp = [&]() -> bool {
+      auto do_dp = [&](uint32_t db) -> bool {  // into buffer db
         if (!wait(&bar->b2_full[d_st.i], d_st.ph)) return false;
         if (--d_left == 0) {
           if (d_last < BN) clear_rows(sB + d_st.i * 2 * C::B_BYTES + C::B_BYTES, d_last);
           next_range(d_second, d_left, d_last);
         }
         tc_fence_after();
-        issue_scores(tmem_base + C::TM_DP, tmem_base + C::TM_A2, a2, sB0 + d_st.i * 2 * C::B_BYTES + C::B_BYTES,
-                     bx0 + ((d_st.i * 2 + 1) * C::BX_BYTES >> 4), &bar->dp_full);
+        issue_scores(tmem_base + C::TM_DP + (C::DB ? db * BN : 0u), tmem_base + C::TM_A2, a2, sB0 + d_st.i * 2 * C::B_BYTES + C::B_BYTES,
+                     bx0 + ((d_st.i * 2 + 1) * C::BX_BYTES >> 4), &bar->dp_full[C::DB ? db : 0u]);
         if (!KV) commit(&bar->b2_empty[d_st.i]);
         d_st.next();
         return true;
       };
-      if (!do_s() || !do_dp()) break;
+      if (!do_s() || !do_dp(ph)) break;
       bool ok = true;
-      for (int left = n; left > 0; --left, ph ^= 1u) {
+      for (int left = n; left > 0; --left, ph2 ^= ph, ph ^= 1u) {
+        const uint32_t db = C::DB ? ph : 0u, ds_ph = C::DB ? ph2 : ph;
+        const uint32_t t_ds = tmem_base + C::TM_DP + db * BN;
         const bool more = left > 1, first = left == n - pre;  // (first to accumulate)
         const uint32_t b1 = sB0 + c_st.i * 2 * C::B_BYTES + dh_off, b2 = b1 + C::B_BYTES;
         if (!C::ATM && !more) commit(&bar->a_empty);  // every S and dP of the item is issued
@@ -791,6 +798,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         const bool early = kEarlyS && !(KV && few);
         if (kEarlyS && STAGES > 1) {
           if (!wait(&bar->s_free, ph) || (early && more && !do_s())) { ok = false; break; }
+          // (The other buffer's dS was read by the accumulation issued last.)
+          if (C::DB && more && !do_dp(ph ^ 1u)) { ok = false; break; }
         }
         if (first) {
           if (!wait(&bar->acc_empty, acc_ph)) { ok = false; break; }
@@ -803,16 +812,16 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         }
         if (!early && STAGES > 1 && more && !do_s()) { ok = false; break; }
         if (!KV && left > n - pre) {  // delta only: dP is read, B1 is free
-          if (!wait(bar->ds_full, ph)) { ok = false; break; }
+          if (!wait(&bar->ds_full[db], ds_ph)) { ok = false; break; }
           commit(&bar->b1_empty[c_st.i]);
-        } else if (!issue_acc(bar->ds_full, ph, tmem_base + C::TM_ACC2, tmem_base + C::TM_DP, C::NC, rest_ds, b1,
-                              !first, &bar->b1_empty[c_st.i])) {
+        } else if (!issue_acc(&bar->ds_full[db], ds_ph, tmem_base + C::TM_ACC2, t_ds, C::NC,
+                              few ? t_ds + C::NC / 2 : 0, b1, !first, &bar->b1_empty[c_st.i])) {
           ok = false;
           break;
         }
         c_st.next();
         if (more) {
-          if ((STAGES == 1 && !do_s()) || !do_dp()) { ok = false; break; }
+          if ((STAGES == 1 && !do_s()) || (!C::DB && !do_dp(ph ^ 1u))) { ok = false; break; }
         } else {
           commit(&bar->acc_full);
         }
@@ -826,11 +835,15 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     constexpr int NC = C::NC;
     const uint32_t tS = tmem_base + lane_off + C::TM_S + g * NC;
-    const uint32_t tDP = tmem_base + lane_off + C::TM_DP + g * NC;
+    const uint32_t tDP0 = tmem_base + lane_off + C::TM_DP + g * NC;
     const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
     constexpr float kInv = BwdScale<BF16>::kInv;
     const F2 sl2_2 = f2(p.scale_log2, p.scale_log2), kinv_2 = f2(kInv, kInv);
-    uint32_t ph = 0, acc_ph = 0, aload = 0, sums = 0;
+    uint32_t ph = 0, ph2 = 0, acc_ph = 0, aload = 0, sums = 0;  // ph2: of a barrier that every other tile uses (DB)
+    auto next_tile = [&]() {
+      ph2 ^= ph;
+      ph ^= 1u;
+    };
     auto arrive = [&](uint64_t* b) {
       tc_fence_before();
       __syncwarp();
@@ -907,6 +920,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       // there; and apart the items of few terms, of which some sum delta themselves.)
       auto tile = [&](auto first, auto few, int i) -> bool {
         constexpr bool kFew = decltype(few)::value;
+        const uint32_t db = C::DB ? ph : 0u, tDP = tDP0 + db * BN;
         if (!wait(&bar->s_full, ph)) return false;
         tc_fence_after();
         uint32_t x[NC];
@@ -950,7 +964,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             }
           }
         }
-        if (!wait(&bar->dp_full, ph)) return false;
+        if (!wait(&bar->dp_full[db], C::DB ? ph2 : ph)) return false;
         tc_fence_after();
         ld(tDP, x);
         if constexpr (!KV && kFew) {
@@ -976,8 +990,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
               }
             }
             if (i < pre) {
-              arrive(bar->ds_full);
-              ph ^= 1u;
+              arrive(&bar->ds_full[db]);
+              next_tile();
               return true;
             }
           }
@@ -994,9 +1008,9 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             if constexpr (kFew) pk2[c] = pack_rest<BF16>(d, pk[c]);
           }
           if constexpr (kFew) put(tDP + NC / 2, pk2, h);
-          give(tDP, pk, h, bar->ds_full);
+          give(tDP, pk, h, &bar->ds_full[db]);
         }
-        ph ^= 1u;
+        next_tile();
         return true;
       };
       using Yes = std::true_type;
