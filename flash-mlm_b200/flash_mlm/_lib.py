@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -169,6 +170,25 @@ class QkRopeArgs(ctypes.Structure):
     ]
 
 
+def packer(cls):
+    """A function of the fields of `cls` in their order (a view as its seven) that gives the struct's bytes: of a
+    call's argument block, half the host time of setting its fields (4 of 8 us for the backward pass)."""
+    codes = {ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P", ctypes.c_size_t: "N"}
+    flat = [t for _, t in cls._fields_]
+    flat = [t for f in flat for t in ([x for _, x in f._fields_] if issubclass(f, ctypes.Structure) else [f])]
+    s = struct.Struct("@" + "".join(codes[t] for t in flat) + "0P")
+    if s.size != ctypes.sizeof(cls):
+        raise AssertionError(f"{cls.__name__}: packed size {s.size}, struct {ctypes.sizeof(cls)}")
+    return s.pack
+
+
+pack_dense_args = packer(DenseArgs)
+pack_packed_args = packer(PackedArgs)
+pack_attn_bwd_args = packer(AttnBwdArgs)
+pack_qk_rope_args = packer(QkRopeArgs)
+NO_VIEW = (0,) * 7
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -195,17 +215,17 @@ def lib() -> ctypes.CDLL:
         L.fmlm_attn_packed_fwd.restype = ctypes.c_int
         L.fmlm_attn_packed_fwd_noalloc.argtypes = [ctypes.POINTER(PackedArgs), vp]
         L.fmlm_attn_packed_fwd_noalloc.restype = ctypes.c_int
-        L.fmlm_attn_dense_fwd_lse.argtypes = [ctypes.POINTER(DenseArgs), i32, vp, vp]
+        L.fmlm_attn_dense_fwd_lse.argtypes = [vp, i32, vp, vp]  # (vp: a struct by reference, or its bytes)
         L.fmlm_attn_dense_fwd_lse.restype = ctypes.c_int
-        L.fmlm_attn_packed_fwd_lse.argtypes = [ctypes.POINTER(PackedArgs), i32, vp, vp]
+        L.fmlm_attn_packed_fwd_lse.argtypes = [vp, i32, vp, vp]
         L.fmlm_attn_packed_fwd_lse.restype = ctypes.c_int
-        L.fmlm_attn_bwd.argtypes = [ctypes.POINTER(AttnBwdArgs), vp]
+        L.fmlm_attn_bwd.argtypes = [vp, vp]
         L.fmlm_attn_bwd.restype = ctypes.c_int
         L.fmlm_attn_bwd_workspace_bytes.argtypes = [i64]
         L.fmlm_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
-        L.fmlm_qk_rope_fwd.argtypes = [ctypes.POINTER(QkRopeArgs), vp]
+        L.fmlm_qk_rope_fwd.argtypes = [vp, vp]
         L.fmlm_qk_rope_fwd.restype = ctypes.c_int
-        L.fmlm_qk_rope_bwd.argtypes = [ctypes.POINTER(QkRopeArgs), vp]
+        L.fmlm_qk_rope_bwd.argtypes = [vp, vp]
         L.fmlm_qk_rope_bwd.restype = ctypes.c_int
         L.fmlm_qk_rope_bwd_workspace_bytes.argtypes = [i32]
         L.fmlm_qk_rope_bwd_workspace_bytes.restype = ctypes.c_size_t

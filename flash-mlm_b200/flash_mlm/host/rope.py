@@ -9,8 +9,6 @@ in q, k and the norm's weights.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from flash_mlm import _lib
@@ -56,14 +54,14 @@ def _rows_ready(x: torch.Tensor) -> torch.Tensor:
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _view(x: torch.Tensor) -> _lib.View4:
+def _view(x: torch.Tensor) -> tuple[int, ...]:
     if x.ndim == 4:
         b, h, n, _ = x.shape
         sb, sh, sn, _ = x.stride()
-        return _lib.View4(x.data_ptr(), n, h, b, sn, sh, sb)
+        return x.data_ptr(), n, h, b, sn, sh, sb
     h, t, _ = x.shape
     sh, st, _ = x.stride()
-    return _lib.View4(x.data_ptr(), t, h, 1, st, sh, 0)
+    return x.data_ptr(), t, h, 1, st, sh, 0
 
 
 def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
@@ -128,39 +126,37 @@ def _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, position
             raise ValueError("all tensors must be on q's device")
 
 
-def _args(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets):
-    """The argument block of a call, and the tensors it points into."""
-    a = _lib.QkRopeArgs()
+def _launch(fn, what, call, q, k, out_q, out_k, gq=None, gk=None, dwq=None, dwk=None):
+    """One kernel call: `call` holds the arguments of ``qk_norm_rope`` behind q and k."""
+    rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets = call
     packed = q.ndim == 3
-    a.dtype, a.head_dim, a.packed = _lib.dtype_code(q.dtype), q.shape[-1], int(packed)
-    a.batch, a.seq_len = (q_meta.B, max(q_meta.N, 1)) if packed else (q.shape[0], q.shape[2])
-    a.q_heads, a.k_heads = q.shape[-3], k.shape[-3]
-    a.normalize, a.eps = int(normalize), float(eps)
-    a.q, a.k = _view(q), _view(k)
-    keep = [q, k]
+    keep = []  # contiguous copies, alive until the launch
 
-    def ptr(x, dtype=None):
+    def ptr(x):
         if x is None:
-            return None
+            return 0
         if not x.is_contiguous():
             x = x.detach().contiguous()
-        keep.append(x)
+            keep.append(x)
         return x.data_ptr()
 
+    batch, seq_len = (q_meta.B, max(q_meta.N, 1)) if packed else (q.shape[0], q.shape[2])
     w = q_weight if q_weight is not None else k_weight
-    a.weight_f32 = int(w is None or w.dtype == torch.float32)
-    a.q_weight, a.k_weight = ptr(q_weight), ptr(k_weight)
-    if rotary is not None:
-        a.rotary_dim, a.pairs, a.max_positions = rotary.rotary_dim, _PAIRS[rotary.pairs], rotary.max_positions
-        a.table = rotary.table.data_ptr()
-        a.positions, a.position_offsets = ptr(positions), ptr(position_offsets)
-    if q_meta is not None:
-        if packed:
-            a.token_indices = ptr(q_meta.token_indices)
-        else:
-            a.lengths = ptr(q_meta.lengths)
-    a.error_word = _lib.error_word(q.device).data_ptr()
-    return a, keep
+    weight_f32 = int(w is None or w.dtype == torch.float32)
+    turn = (0, 0, 0) if rotary is None else (rotary.rotary_dim, _PAIRS[rotary.pairs], rotary.max_positions)
+    lengths, tokens = (None, None) if q_meta is None else (None, q_meta.token_indices) if packed else (q_meta.lengths, None)
+    ws = None
+    if dwq is not None or dwk is not None:
+        ws = torch.empty(_lib.lib().fmlm_qk_rope_bwd_workspace_bytes(q.shape[-1]), dtype=torch.uint8, device=q.device)
+    args = _lib.pack_qk_rope_args(
+        _lib.dtype_code(q.dtype), q.shape[-1], int(packed), batch, seq_len, q.shape[-3], k.shape[-3], int(normalize),
+        weight_f32, *turn, float(eps), *_view(q), *_view(k),
+        *(_lib.NO_VIEW if gq is None else _view(gq)), *(_lib.NO_VIEW if gk is None else _view(gk)),
+        ptr(q_weight), ptr(k_weight), 0 if rotary is None else rotary.table.data_ptr(),
+        ptr(positions), ptr(position_offsets), ptr(lengths), ptr(tokens), out_q.data_ptr(), out_k.data_ptr(),
+        0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
+        0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _lib.error_word(q.device).data_ptr())
+    _lib.launch(fn, q.device, what, args)
 
 
 def _outputs(q, k):
@@ -171,10 +167,7 @@ def _outputs(q, k):
 def _forward(q, k, *call):
     out_q, out_k = _outputs(q, k)
     if q.numel() and k.numel():
-        a, keep = _args(_rows_ready(q), _rows_ready(k), *call)
-        a.q_out, a.k_out = out_q.data_ptr(), out_k.data_ptr()
-        _lib.launch(_lib.lib().fmlm_qk_rope_fwd, q.device, "qk_norm_rope", ctypes.byref(a))
-        del keep
+        _launch(_lib.lib().fmlm_qk_rope_fwd, "qk_norm_rope", call, _rows_ready(q), _rows_ready(k), out_q, out_k)
     return out_q, out_k
 
 
@@ -202,18 +195,9 @@ def _rope_backward(ctx, gq, gk):
             if w is not None:
                 w.zero_()
         return dq, dk, dwq, dwk, None, None, None, None, None, None
-    a, keep = _args(_rows_ready(q), _rows_ready(k), rotary, q_weight, k_weight, normalize, eps, q_meta, positions,
-                    position_offsets)
-    gq, gk = _rows_ready(gq), _rows_ready(gk)
-    a.gq, a.gk = _view(gq), _view(gk)
-    a.q_out, a.k_out = dq.data_ptr(), dk.data_ptr()
-    if dwq is not None or dwk is not None:
-        a.dq_weight, a.dk_weight = (None if w is None else w.data_ptr() for w in (dwq, dwk))
-        nbytes = _lib.lib().fmlm_qk_rope_bwd_workspace_bytes(q.shape[-1])
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.launch(_lib.lib().fmlm_qk_rope_bwd, q.device, "qk_norm_rope backward", ctypes.byref(a))
-    del keep
+    call = (rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
+    _launch(_lib.lib().fmlm_qk_rope_bwd, "qk_norm_rope backward", call, _rows_ready(q), _rows_ready(k), dq, dk,
+            _rows_ready(gq), _rows_ready(gk), dwq, dwk)
     return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 

@@ -24,8 +24,6 @@ the same bits.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from flash_mlm import _lib
@@ -44,15 +42,15 @@ def _tma_ready(x: torch.Tensor) -> torch.Tensor:
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-def _view(x: torch.Tensor) -> _lib.View4:
-    """[B, H, N, D] or [H, T, D] as a [batch][heads][rows] view."""
+def _view(x: torch.Tensor) -> tuple[int, ...]:
+    """[B, H, N, D] or [H, T, D] as the fields of a [batch][heads][rows] view."""
     if x.ndim == 4:
         b, h, n, _ = x.shape
         sb, sh, sn, _ = x.stride()
-        return _lib.View4(x.data_ptr(), n, h, b, sn, sh, sb)
+        return x.data_ptr(), n, h, b, sn, sh, sb
     h, t, d = x.shape
     sh, st, _ = x.stride()
-    return _lib.View4(x.data_ptr(), t, h, 1, st, sh, h * t * d)
+    return x.data_ptr(), t, h, 1, st, sh, h * t * d
 
 
 def _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal):
@@ -158,39 +156,30 @@ def _forward(layout, q, k, v, scale, q_meta, context_k, context_v, context_meta,
     q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
     h, d, hk = q.shape[-3], q.shape[-1], k.shape[-3]
     L = _lib.lib()
-    err = _lib.error_word(q.device)
+    code, err = _lib.dtype_code(q.dtype), _lib.error_word(q.device).data_ptr()
+    views = (*_view(q), *_view(k), *_view(v))
     if layout == _lib.FMLM_BWD_DENSE:
-        args = _lib.DenseArgs()
-        args.dtype, args.head_dim = _lib.dtype_code(q.dtype), d
-        args.batch, args.num_heads, args.seq_len = q.shape[0], h, q.shape[2]
-        args.context_batch_size = 1
-        args.scale = float(scale)
-        args.q, args.k, args.v = _view(q), _view(k), _view(v)
-        args.out, args.error_word = out.data_ptr(), err.data_ptr()
+        args = _lib.pack_dense_args(
+            code, d, q.shape[0], h, q.shape[2], 0, 0, 1, 0, float(scale),  # no MLA, no prefill, no context
+            *views, *_lib.NO_VIEW, *_lib.NO_VIEW, out.data_ptr(), err)
         launch = L.fmlm_attn_dense_fwd_lse
     else:
         packed = layout == _lib.FMLM_BWD_PACKED
-        args = _lib.PackedArgs()
-        args.dtype, args.head_dim, args.num_heads, args.batch = _lib.dtype_code(q.dtype), d, h, q_meta.B
-        args.causal_query_seq_attn = int(causal)
-        args.context_batch_size = 1
-        args.scale = float(scale)
-        args.q_layout = args.kv_layout = _lib.FMLM_LAYOUT_PACKED if packed else _lib.FMLM_LAYOUT_PADDED
-        args.seq_len = 0 if packed else q.shape[2]
-        args.total_q_len = q_meta.total_tokens
-        args.q, args.k, args.v = _view(q), _view(k), _view(v)
-        args.cu_seqlens_q = q_meta.cu_seqlens.data_ptr()
+        rows = _lib.FMLM_LAYOUT_PACKED if packed else _lib.FMLM_LAYOUT_PADDED
+        ctx_bs, kc, vc, cu_kv = 1, _lib.NO_VIEW, _lib.NO_VIEW, 0
         if context_k is not None and context_meta.total_tokens > 0:
             context_k, context_v = _tma_ready(context_k), _tma_ready(context_v)
-            args.k_cache, args.v_cache = _view(context_k), _view(context_v)
-            args.cu_seqlens_kv = context_meta.cu_seqlens.data_ptr()
-            args.context_batch_size = context_meta.B
-        args.out, args.out_rows_per_head, args.out_padded = out.data_ptr(), q_meta.total_tokens, int(not packed)
-        nbytes = L.fmlm_packed_workspace_bytes(q_meta.B, q_meta.total_tokens, d)
+            ctx_bs, kc, vc, cu_kv = context_meta.B, _view(context_k), _view(context_v), context_meta.cu_seqlens.data_ptr()
+        total = q_meta.total_tokens
+        nbytes = L.fmlm_packed_workspace_bytes(q_meta.B, total, d)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        args.workspace, args.workspace_bytes, args.error_word = ws.data_ptr(), nbytes, err.data_ptr()
+        args = _lib.pack_packed_args(
+            code, d, h, q_meta.B, 0, 0, int(causal), ctx_bs, float(scale),  # no MLA, no prefill
+            rows, rows, 0 if packed else q.shape[2], total, *views, *kc, *vc,
+            q_meta.cu_seqlens.data_ptr(), cu_kv, out.data_ptr(), total, ws.data_ptr(), nbytes, err,
+            0, 0, int(not packed))  # a new schedule, no context_index, padded output
         launch = L.fmlm_attn_packed_fwd_lse
-    _lib.launch(launch, q.device, "flash_attn_mlm_fwd", ctypes.byref(args), hk, lse.data_ptr())
+    _lib.launch(launch, q.device, "flash_attn_mlm_fwd", args, hk, lse.data_ptr())
     return out, lse
 
 
@@ -251,29 +240,21 @@ def _backward(layout, dout, q, k, v, out, lse, scale, q_meta, context_k, context
     dout, out, lse = _tma_ready(dout.contiguous()), _tma_ready(out.contiguous()), lse.contiguous()
     packed = layout == _lib.FMLM_BWD_PACKED
     L = _lib.lib()
-    args = _lib.AttnBwdArgs()
-    args.dtype, args.head_dim, args.layout = _lib.dtype_code(q.dtype), q.shape[-1], layout
-    args.batch = q_meta.B if packed else q.shape[0]
-    args.num_heads, args.kv_heads = q.shape[-3], k.shape[-3]
-    args.seq_len = 0 if packed else q.shape[2]
-    args.causal_query_seq_attn = int(causal)
-    args.scale = float(scale)
-    args.total_q_len = q.shape[1] if packed else 0
-    args.q, args.k, args.v, args.dout = _view(q), _view(k), _view(v), _view(dout)
-    if q_meta is not None:
-        args.cu_seqlens_q = q_meta.cu_seqlens.data_ptr()
+    entries, rows_c, kc, vc, cu_kv = 0, 0, _lib.NO_VIEW, _lib.NO_VIEW, 0
     if context_k is not None and context_meta.total_tokens > 0:
         context_k, context_v = _tma_ready(context_k), _tma_ready(context_v)
-        args.context_entries, args.total_context_len = context_meta.B, context_meta.total_tokens
-        args.k_context, args.v_context = _view(context_k), _view(context_v)
-        args.cu_seqlens_context = context_meta.cu_seqlens.data_ptr()
-    args.out, args.lse = out.data_ptr(), lse.data_ptr()
-    args.dq, args.dk, args.dv, args.dk_context, args.dv_context = (None if g is None else g.data_ptr() for g in grads)
+        entries, rows_c, cu_kv = context_meta.B, context_meta.total_tokens, context_meta.cu_seqlens.data_ptr()
+        kc, vc = _view(context_k), _view(context_v)
     nbytes = L.fmlm_attn_bwd_workspace_bytes(lse.numel())
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-    args.error_word = _lib.error_word(dev).data_ptr()
-    _lib.launch(L.fmlm_attn_bwd, dev, "flash_attn_mlm_bwd", ctypes.byref(args))
+    args = _lib.pack_attn_bwd_args(
+        _lib.dtype_code(q.dtype), q.shape[-1], layout, q_meta.B if packed else q.shape[0], q.shape[-3], k.shape[-3],
+        0 if packed else q.shape[2], int(causal), entries, float(scale), q.shape[1] if packed else 0, rows_c,
+        *_view(q), *_view(k), *_view(v), *_view(dout), *kc, *vc, out.data_ptr(), lse.data_ptr(),
+        0 if q_meta is None else q_meta.cu_seqlens.data_ptr(), cu_kv,
+        *[0 if g is None else g.data_ptr() for g in grads],  # dq, dk, dv and the context's
+        ws.data_ptr(), nbytes, _lib.error_word(dev).data_ptr())
+    _lib.launch(L.fmlm_attn_bwd, dev, "flash_attn_mlm_bwd", args)
     return grads
 
 
