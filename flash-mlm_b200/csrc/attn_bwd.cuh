@@ -40,10 +40,10 @@
 // (factor 1.0; all items that way would add 2 to the 7 matrix products).
 //
 // What bounds it: the tensor pipe at head_dim 128 (16 heads of 8192 tokens,
-// bf16: Q pass 626 us, 1317 TFLOP/s; KV pass 721 us, 1525 TFLOP/s, 71 % of the
+// bf16: Q pass 629 us, 1310 TFLOP/s; KV pass 728 us, 1511 TFLOP/s, 71 % of the
 // tensor cycles), the chain exponentials - TMEM - MMA at head_dim 64 (2 x 16
-// heads of 2048 tokens: 79 and 88 us, tensor pipe 39 and 53 %, exponentials'
-// unit 51 and 47 %).
+// heads of 2048 tokens: 75 and 88 us, tensor pipe 39 and 53 %, exponentials'
+// unit 52 and 47 %).
 //
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
