@@ -157,7 +157,8 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
     return set_error(FMLM_ERR_INVALID, "out and lse are required; out and dout must be 16-byte aligned");
   if (!aligned32(a->dq) || !aligned32(a->dk) || !aligned32(a->dv))
     return set_error(FMLM_ERR_INVALID, "dq, dk, dv must be 32-byte aligned");
-  // float16: lse in units of the scores has to fit three float16 numbers
+  // float16: lse in units of q k^T has to fit the float16 columns (the KV pass
+  // reports a row's that does not); a smaller scale would shift log(keys) out.
   const bool bf16 = a->dtype == FMLM_DTYPE_BF16;
   const float mag = std::fabs(a->scale);
   if (!(mag <= (bf16 ? 0x1p64f : 0x1p20f)) || (!bf16 && mag < 0x1p-24f))
@@ -197,14 +198,12 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   // and its scales are refused above instead.
   const float sl2 = a->scale * 1.4426950408889634f;
   p.scale_log2 = std::fabs(sl2) < 0x1p-100f ? 0x1p-100f : sl2;
-  // A power of two near 1 / scale_log2 (float16 holds 2^-14 .. 2^15), so that
-  // what the 16-bit columns hold is of lse's own magnitude.
-  const int e = std::min(bf16 ? 100 : 15, std::max(bf16 ? -100 : -14, -std::ilogb(p.scale_log2)));
-  p.ext_unit = std::ldexp(1.f, e);
+  // bfloat16: a power of two near 1 / scale_log2, so that what the columns hold
+  // is of lse's own magnitude.  float16's columns have their units.
+  p.ext_unit = bf16 ? std::ldexp(1.f, std::min(100, std::max(-100, -std::ilogb(p.scale_log2)))) : 1.f;
   const float ext_mul = 1.f / (p.scale_log2 * p.ext_unit);
-  // -400 in the exponent; one 16-bit number is near enough
-  const float none = -400.f * ext_mul;
-  p.xnone = make_uint4(bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(none)) : __half_as_ushort(__float2half_rn(none)), 0, 0, 0);
+  // -400 in the exponent; at float16's smallest scales what the columns hold unsaturated, -92 or less
+  p.none = bf16 ? -400.f * ext_mul : std::copysign(std::min(400.f * std::fabs(ext_mul), 0x1p30f), -ext_mul);
   p.err = a->error_word;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -21,8 +21,8 @@
 // 128 KB per tile through a 128-byte-a-cycle port (measured: 1800 + 1800 cycles
 // a tile for P and dS against 1000 + 650 in the Q pass).  Instead one more K
 // step of the score MMAs adds them: B gets 16 more columns that hold -lse (in
-// units of the scores) and -delta as sums of three 16-bit numbers, A the
-// matching constants, so S and dP arrive with them subtracted.
+// units of the scores) and -delta as sums of three or four 16-bit numbers, A
+// the units of these, so S and dP arrive with them subtracted (ext_columns).
 //
 // delta is dO * O with O as the forward pass returned it, in 16 bits.  Over many
 // keys that costs little (dq, dk within 1.5 of the error of gradients that are
@@ -58,6 +58,8 @@
 
 namespace fmlm {
 
+constexpr int kErrStatistics = 7;
+
 struct BwdParams {
   int layout;  // FMLM_BWD_*
   int B, H, HK, G, N;
@@ -70,11 +72,11 @@ struct BwdParams {
   const int* cu_c;
   const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta}
   uint4* xstats;        // the same as what the KV pass puts into B's extra columns
-  uint4 xnone;          // xstats of a row that is not there: P = 2^-400 = 0, delta = 0
+  float none;           // KV: -lse, as the columns hold it, of a row that is not there: P = 0
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
   float scale, scale_log2;  // scale_log2: of the scores in the exponent (never 0: see the host code)
-  float ext_unit;           // KV: A's constant (a power of two) for the lse columns
+  float ext_unit;           // KV, bfloat16: unit (a power of two) of the lse columns
   int* err;
   unsigned long long timeout_ns;
 };
@@ -395,28 +397,56 @@ __device__ __forceinline__ uint8_t* ext_row(uint8_t* tile, int r, int h) {
   return tile + r * 32 + ((h ^ ((r >> 2) & 1)) << 4);
 }
 
-// v as the sum of three 16-bit numbers (to 2^-27 of it in bfloat16, 2^-33 in
-// float16), float16's saturated.
+// The extra columns' units (A's constants): four columns of B1 for lse, three
+// of B2 for delta.  bfloat16 has float32's exponents, so three numbers of one
+// unit hold a value to 2^-27 of it.  float16 has not: its units fall by 2^11
+// or 2^12, the bits of one number.  lse, in units of q k^T, fits to 2^-36 of it
+// or 2^-39, whichever is larger, up to 65504 * 2^15; delta to 2^-36 of it or
+// 2^-37, up to 65504 * 2^12.  What is larger saturates, and the KV pass says so.
 template <bool BF16>
-__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
-  if constexpr (BF16) {
-    a = __bfloat162float(__float2bfloat16_rn(v));
-    b = __bfloat162float(__float2bfloat16_rn(v - a));
-  } else {
-    a = __half2float(__float2half_rn(fminf(fmaxf(v, -65504.f), 65504.f)));
-    b = __half2float(__float2half_rn(fminf(fmaxf(v - a, -65504.f), 65504.f)));
-  }
-  c = v - a - b;
-  if constexpr (!BF16) c = fminf(fmaxf(c, -65504.f), 65504.f);
+__device__ __forceinline__ uint4 ext_units(float bf16_unit) {
+  if constexpr (BF16)
+    return make_uint4(pack2<BF16>(bf16_unit, bf16_unit), pack2<BF16>(bf16_unit, 0.f), pack2<BF16>(1.f, 1.f), pack2<BF16>(1.f, 0.f));
+  else
+    return make_uint4(pack2<BF16>(0x1p15f, 0x1p4f), pack2<BF16>(0x1p-7f, 0x1p-14f), pack2<BF16>(0x1p12f, 1.f), pack2<BF16>(0x1p-12f, 0.f));
 }
 
-// The extra columns of a row: three of B1 (lse) in x, y; three of B2 (delta) in z, w.
+// The float16 number of this unit that v is nearest to, taken off v (exactly).
+// Saturates; of infinities and NaN it makes NaN.
+__device__ __forceinline__ float take_half(float& v, float unit) {
+  const float c = __half2float(__float2half_rn(fminf(fmaxf(v / unit, -65504.f), 65504.f) + (v - v)));
+  v = fmaf(-c, unit, v);
+  return c;
+}
+
+// The extra columns of a row: four of B1 (lse) in x, y; three of B2 (delta) in z, w.
 template <bool BF16>
 __device__ __forceinline__ uint4 ext_columns(float nl, float nd) {
-  float a, b, c, d, e, f;
-  split3<BF16>(nl, a, b, c);
-  split3<BF16>(nd, d, e, f);
-  return make_uint4(pack2<BF16>(a, b), pack2<BF16>(c, 0.f), pack2<BF16>(0.f, d), pack2<BF16>(e, f));
+  float l[4], d[3];
+  if constexpr (BF16) {
+    auto split3 = [](float v, float* o) {
+      o[0] = __bfloat162float(__float2bfloat16_rn(v));
+      o[1] = __bfloat162float(__float2bfloat16_rn(v - o[0]));
+      o[2] = v - o[0] - o[1];
+    };
+    split3(nl, l);
+    split3(nd, d);
+    l[3] = 0.f;
+  } else {
+    l[0] = take_half(nl, 0x1p15f);
+    l[1] = take_half(nl, 0x1p4f);
+    l[2] = take_half(nl, 0x1p-7f);
+    l[3] = take_half(nl, 0x1p-14f);
+    d[0] = take_half(nd, 0x1p12f);
+    d[1] = take_half(nd, 1.f);
+    d[2] = take_half(nd, 0x1p-12f);
+  }
+  return make_uint4(pack2<BF16>(l[0], l[1]), pack2<BF16>(l[2], l[3]), pack2<BF16>(d[0], d[1]), pack2<BF16>(d[2], 0.f));
+}
+
+// float16: the columns' first numbers are at their end (or past it).
+__device__ __forceinline__ bool ext_saturated(const uint4& x) {
+  return (x.x & 0x7fffu) == 0x7bffu || (x.z & 0x7fffu) == 0x7bffu;
 }
 
 template <int D, bool KV, bool BF16>
@@ -473,11 +503,10 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     tmem_relinquish();
   }
   if constexpr (KV) {
-    // Rows of 32 bytes in the 32-byte swizzle.  A's: the unit of the lse
-    // columns three times, 1 three times, zeros; B's second halves: zeros.
+    // Rows of 32 bytes in the 32-byte swizzle.  A's: the columns' units, then
+    // zeros; B's second halves: zeros.
     for (int r = threadIdx.x; r < C::BM; r += C::THREADS) {
-      const uint32_t u = pack2<BF16>(p.ext_unit, p.ext_unit), um = pack2<BF16>(p.ext_unit, 1.f), o = pack2<BF16>(1.f, 1.f);
-      *reinterpret_cast<uint4*>(ext_row(sAx, r, 0)) = make_uint4(u, um, o, 0);
+      *reinterpret_cast<uint4*>(ext_row(sAx, r, 0)) = ext_units<BF16>(p.ext_unit);
       *reinterpret_cast<uint4*>(ext_row(sAx, r, 1)) = make_uint4(0, 0, 0, 0);
     }
     for (int r = threadIdx.x; r < 2 * STAGES * BN; r += C::THREADS)
@@ -608,6 +637,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   } else if (KV && warp == C::EXT_WARP) {
     // ------------------------------------------------------------ extra columns
     // Loaded one tile ahead: the stage is waited for with the values in hand.
+    const uint4 none = ext_columns<BF16>(p.none, 0.f);
     uint32_t fill = 0;
     for (uint32_t ring = 0;; ++ring) {
       const BwdItem* slot = take_item(ring);
@@ -621,7 +651,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
           const int r = row0 + t * BN + c * 32 + lane;
-          x[c] = r < end0 ? __ldg(src + r) : p.xnone;
+          x[c] = r < end0 ? __ldg(src + r) : none;
         }
         if (++t == nt0) {
           t = 0;
@@ -633,14 +663,17 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         const int st = fill % STAGES;
         if (!wait(&bar->b1_empty[st], ((fill / STAGES) & 1u) ^ 1u)) break;
         uint8_t* x1 = sBx + st * 2 * C::BX_BYTES;
+        bool saturated = false;
 #pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
+          if (!BF16) saturated |= ext_saturated(x[c]);
           *reinterpret_cast<uint4*>(ext_row(x1, c * 32 + lane, 0)) = make_uint4(x[c].x, x[c].y, 0, 0);
-          *reinterpret_cast<uint4*>(ext_row(x1 + C::BX_BYTES, c * 32 + lane, 0)) = make_uint4(0, x[c].z, x[c].w, 0);
+          *reinterpret_cast<uint4*>(ext_row(x1 + C::BX_BYTES, c * 32 + lane, 0)) = make_uint4(0, 0, x[c].z, x[c].w);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar->b1_full[st]);
+        if (saturated) atomicExch(p.err, kErrStatistics);
         if (i + 1 < n) load();
       }
       if (failed) break;

@@ -331,7 +331,8 @@ def check_device_errors(device: torch.device | None = None) -> None:
     context); 4 = a packed sequence had more than 65536 work items (it was
     not computed); 5 = a cache append would have passed the cache capacity
     (nothing was written); 6 = a position lay outside the rotary table (the
-    table's nearest row was used).
+    table's nearest row was used); 7 = float16 scores, before their scale, or
+    output gradients past what the attention's backward pass holds (dk, dv).
     """
     devs = [device] if device is not None else [torch.device("cuda", i) for i in list(_err_words)]
     for d in devs:
@@ -343,7 +344,8 @@ def check_device_errors(device: torch.device | None = None) -> None:
                     3: "met a context_index entry out of range",
                     4: "met a sequence too long for the tile schedule",
                     5: "would have overrun a context cache's capacity (nothing appended)",
-                    6: "met a position outside the rotary table"}.get(v, "failed")
+                    6: "met a position outside the rotary table",
+                    7: "met float16 scores or output gradients too large for dk and dv"}.get(v, "failed")
             raise FlashMLMError(f"flash_mlm kernel on {d} {what} (code {v}); results are invalid")
 
 

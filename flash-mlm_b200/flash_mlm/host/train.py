@@ -67,7 +67,7 @@ def _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal
         raise ValueError("the heads of q must be a multiple of the heads of k and v")
     validate_head_dim_supported(qs[-1])
     half = _lib.dtype_code(q.dtype) == _lib.FMLM_DTYPE_F16
-    # float16: the backward pass holds lse / scale in three float16 numbers
+    # float16: the backward pass holds lse / scale in float16 numbers, up to 2^31
     if not abs(scale) <= (2.0**20 if half else 2.0**64) or (half and abs(scale) < 2.0**-24):
         raise ValueError("scale must be finite, at most 2^64 in magnitude, for float16 in [2^-24, 2^20]")
     packed = q.ndim == 3
@@ -206,6 +206,10 @@ def flash_attn_mlm_bwd(
     tensors' shapes and dtypes, contiguous, with zero rows past each sequence.
     What is not needed (``need_dq``, ``need_dkv``), and the context's without
     a context, is None.
+
+    float16: a row with |lse / scale| of 2^31 or more (scores of that size
+    before they are scaled) has no valid part in dk and dv; the error word says
+    so (``check_device_errors``).
     """
     layout = _validate(q, k, v, scale, q_meta, context_k, context_v, context_meta, causal_query_seq_attn)
     _require_packed(q, context_k, causal_query_seq_attn)

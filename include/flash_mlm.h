@@ -186,7 +186,8 @@ typedef struct fmlm_attn_bwd_args {
   void *dk_context, *dv_context;    /* contiguous [kv_heads][total_context_len][D], 32-byte aligned; rows of no entry are left unwritten */
   void* workspace;                  /* fmlm_attn_bwd_workspace_bytes() bytes, 16-byte aligned */
   size_t workspace_bytes;
-  int32_t* error_word;
+  int32_t* error_word;              /* float16: set to 7 where a row's |lse / scale| reaches 2^31 (or its |sum dout * out|
+                                       2^28), which the pass of dk and dv cannot hold; their values are then invalid */
 } fmlm_attn_bwd_args;
 
 /* Gradients of q, k, v (and of the context's k, v): dq, dk, dv from dout.
