@@ -138,7 +138,8 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   if ((rc = check_view(a->dout, "dout", qr, a->num_heads, qb))) return rc;
   if ((rc = check_view(a->k, "k", qr, a->kv_heads, qb))) return rc;
   if ((rc = check_view(a->v, "v", qr, a->kv_heads, qb))) return rc;
-  if (a->dout.row_stride != D || (a->num_heads > 1 && a->dout.head_stride != qr * D) ||
+  // (a stride along an axis of one says nothing: torch leaves any there)
+  if ((qr > 1 && a->dout.row_stride != D) || (a->num_heads > 1 && a->dout.head_stride != qr * D) ||
       (qb > 1 && a->dout.batch_stride != a->num_heads * qr * D))
     return set_error(FMLM_ERR_INVALID, "dout must be contiguous");
   const bool ctx = a->context_entries > 0 && a->total_context_len > 0;

@@ -27,7 +27,8 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 
 // Encodes a 4-D tiled map {D, rows, heads, batch} over `v` with a box of
 // {swizzle_bytes / 2, box_rows, 1, 1} and the matching shared-memory swizzle.
-// Empty views get a 1-row map over `fallback` that the kernel never loads.
+// Empty views get a 1-row map over `fallback` that the kernel never loads.  The
+// row stride of one row is not looked at.
 inline int encode_view(CUtensorMap* m, const fmlm_view4& v, int D, int box_rows, int dtype, const void* fallback,
                 const char* name) {
   auto enc = encode_fn();
@@ -41,7 +42,7 @@ inline int encode_view(CUtensorMap* m, const fmlm_view4& v, int D, int box_rows,
   dims[1] = empty ? 1 : static_cast<cuuint64_t>(v.rows);
   dims[2] = empty ? 1 : static_cast<cuuint64_t>(v.heads);
   dims[3] = empty ? 1 : static_cast<cuuint64_t>(v.batch);
-  const int64_t rs = empty ? D : v.row_stride;
+  const int64_t rs = empty || v.rows == 1 ? D : v.row_stride;
   int64_t hs = empty ? D : v.head_stride;
   int64_t bs = empty ? D : v.batch_stride;
   if (!empty) {
