@@ -10,6 +10,7 @@ in q, k and the norm's weights.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from flash_mlm import _lib
 from flash_mlm.host.cache import PackMetadata
@@ -233,9 +234,12 @@ def qk_norm_rope(
     the error word (``check_device_errors``).
 
     Returns the new q and k, contiguous, in the layouts and dtype they came in.
-    Differentiable in q, k, q_weight and k_weight.
+    Differentiable in q, k, q_weight and k_weight, in reverse mode (forward-mode
+    tangents are refused).
     """
     _validate(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+    # (Forward-mode tangents belong to tensors that require no gradient: the function refuses them.)
+    graph = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight))
+    if graph or forward_ad._current_level >= 0:
         return _QkNormRope.apply(q, k, q_weight, k_weight, rotary, normalize, eps, q_meta, positions, position_offsets)
     return _forward(q, k, rotary, q_weight, k_weight, normalize, eps, q_meta, positions, position_offsets)
