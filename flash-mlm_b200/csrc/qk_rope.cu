@@ -122,11 +122,10 @@ __device__ __forceinline__ Token locate(const RopeParams& p, long long i) {
   }
   t.pos = 0;
   if (t.valid && p.R > 0) {
-    t.pos = p.positions ? __ldg(p.positions + i) : idx + (p.offsets ? __ldg(p.offsets + seq) : 0);
-    if (t.pos < 0 || t.pos >= p.max_pos) {
-      atomicExch(p.err, kErrPosition);
-      t.pos = t.pos < 0 ? 0 : p.max_pos - 1;
-    }
+    // (an index and an offset may pass 32 bits together)
+    const long long pos = p.positions ? __ldg(p.positions + i) : (long long)idx + (p.offsets ? __ldg(p.offsets + seq) : 0);
+    if (pos < 0 || pos >= p.max_pos) atomicExch(p.err, kErrPosition);
+    t.pos = (int)min(max(pos, 0ll), (long long)p.max_pos - 1);
   }
   return t;
 }
