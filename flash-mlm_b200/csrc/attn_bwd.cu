@@ -1,5 +1,5 @@
 // C-ABI entry point of the attention backward pass: argument checks, tensor
-// maps and the three launches (row statistics, Q pass, KV pass).
+// maps and the launches (row statistics, float16: ranges by sequence, Q pass, KV pass).
 #include <cmath>
 #include <type_traits>
 
@@ -62,21 +62,30 @@ int encode_maps(CUtensorMap* m, const fmlm_attn_bwd_args* a, bool ctx, int qrows
 }
 
 template <int D, bool BF16>
-int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long long rows, cudaStream_t s) {
+int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, cudaStream_t s) {
   using C = BwdCfg<D, false>;
-  const long long vecs = rows * (D / 8);
-  const long long blocks = (vecs + 255) / 256;
-  if (blocks > 0x7fffffffLL) return set_error(FMLM_ERR_INVALID, "problem too large");
+  // A block for every tile of every head; float16: and of v's heads, and of the context's.
+  const long long blocks = (long long)(BF16 ? p.H : p.H + p.HK) * p.slots, cblocks = (long long)p.HK * p.cslots;
+  const long long rblocks = cblocks + ((long long)(p.H + p.HK) * p.B + 3) / 4;
+  if (blocks > 0x7fffffffLL || (!BF16 && rblocks > 0x7fffffffLL)) return set_error(FMLM_ERR_INVALID, "problem too large");
   // Every map before the first launch: a refused view leaves nothing half done.
   const bool ctx = p.C > 0;
   CUtensorMap m[12];
   int rc = encode_maps(m, a, ctx, C::BM, C::BN);
   if (!rc && C::BM != C::BN) rc = encode_maps(m + 6, a, ctx, C::BN, C::BM);
   if (rc) return rc;
+  auto lay = [](const fmlm_view4& v) {
+    return BwdRows{reinterpret_cast<const uint16_t*>(v.data), v.batch_stride, v.head_stride, v.row_stride};
+  };
   attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
-      reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, rows,
-      ext_mul, const_cast<float2*>(p.stats), p.xstats, p.counter);
+      p, reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, ext_mul, lay(a->v));
   rc = check_launch("attn_bwd_stats_kernel");
+  if constexpr (!BF16) {
+    if (!rc && range_by_sequence(p)) {
+      attn_bwd_range_kernel<D><<<(unsigned)rblocks, 128, 0, s>>>(p, lay(a->v_context), (int)cblocks);
+      rc = check_launch("attn_bwd_range_kernel");
+    }
+  }
   // Without dq the Q pass still leaves short rows' delta for the KV pass (where
   // there can be such rows).
   if (!rc && (a->dq || a->layout != FMLM_BWD_DENSE || a->seq_len <= C::BN)) rc = run_pass<D, false, BF16>(m, p, s);
@@ -85,13 +94,13 @@ int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long
 }
 
 template <bool BF16>
-int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, long long rows, cudaStream_t s) {
+int dispatch_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, cudaStream_t s) {
   switch (a->head_dim) {
-    case 16: return run_bwd<16, BF16>(a, p, ext_mul, rows, s);
-    case 32: return run_bwd<32, BF16>(a, p, ext_mul, rows, s);
-    case 64: return run_bwd<64, BF16>(a, p, ext_mul, rows, s);
-    case 128: return run_bwd<128, BF16>(a, p, ext_mul, rows, s);
-    case 256: return run_bwd<256, BF16>(a, p, ext_mul, rows, s);
+    case 16: return run_bwd<16, BF16>(a, p, ext_mul, s);
+    case 32: return run_bwd<32, BF16>(a, p, ext_mul, s);
+    case 64: return run_bwd<64, BF16>(a, p, ext_mul, s);
+    case 128: return run_bwd<128, BF16>(a, p, ext_mul, s);
+    case 256: return run_bwd<256, BF16>(a, p, ext_mul, s);
     default: return set_error(FMLM_ERR_UNSUPPORTED, "HEAD_DIM must be one of {16, 32, 64, 128, 256}");
   }
 }
@@ -112,7 +121,7 @@ int check_view(const fmlm_view4& v, const char* name, int64_t rows, int64_t head
 using namespace fmlm;
 
 extern "C" size_t fmlm_attn_bwd_workspace_bytes(int64_t rows) {
-  return kCounterBytes + (size_t)(rows > 0 ? rows : 0) * (sizeof(float2) + sizeof(uint4));
+  return kCounterBytes + (size_t)(rows > 0 ? rows : 0) * (sizeof(float2) + sizeof(uint4) + sizeof(int4));
 }
 
 extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
@@ -187,7 +196,8 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.cu_c = a->cu_seqlens_context;
   p.counter = reinterpret_cast<int*>(a->workspace);
   p.xstats = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a->workspace) + kCounterBytes);
-  p.stats = reinterpret_cast<const float2*>(p.xstats + rows);
+  p.range = reinterpret_cast<int4*>(p.xstats + rows);
+  p.stats = reinterpret_cast<const float2*>(p.range + rows);
   p.dq = a->dq;
   p.dk = a->dk;
   p.dv = a->dv;
@@ -208,5 +218,5 @@ extern "C" int fmlm_attn_bwd(const fmlm_attn_bwd_args* a, void* stream) {
   p.err = a->error_word;
   p.timeout_ns = kTimeoutNs;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return bf16 ? dispatch_bwd<true>(a, p, ext_mul, rows, s) : dispatch_bwd<false>(a, p, ext_mul, rows, s);
+  return bf16 ? dispatch_bwd<true>(a, p, ext_mul, s) : dispatch_bwd<false>(a, p, ext_mul, s);
 }

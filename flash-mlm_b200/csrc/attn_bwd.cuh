@@ -39,6 +39,15 @@
 // that the first leaves free, for another K walk of the accumulating MMAs
 // (factor 1.0; all items that way would add 2 to the 7 matrix products).
 //
+// float16 P is held times 2^12 (P <= 1), and dS times a power of two that brings
+// its bound |dO| |v| + |delta| to 2^15: as it is, dS of long rows or of small dO
+// would lie among float16's subnormals (4096 keys, dO of 1e-3: dq and dk 8 times
+// as far off as gradients rounded once, now 1.4), and dS of large dO past its
+// end.  A Q item's rows have each their own power, from the row's dO and the
+// largest v that it sees; a KV item one, from its sequence's v and the dO and
+// delta that stream past.  The statistics kernel leaves each tile's largest, so
+// that none depends on rows it does not see.
+//
 // What bounds it: the tensor pipe at head_dim 128 (16 heads of 8192 tokens,
 // bf16: Q pass 629 us, 1310 TFLOP/s; KV pass 728 us, 1511 TFLOP/s, 71 % of the
 // tensor cycles), the chain exponentials - TMEM - MMA at head_dim 64 (2 x 16
@@ -48,7 +57,8 @@
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
 // warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs,
-// warp 18 (KV) copies the streamed rows' extra columns.
+// warp 18 (KV) copies the streamed rows' extra columns, warp 19 (KV, float16)
+// finds dS's power of two.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -71,7 +81,11 @@ struct BwdParams {
   const int* cu_q;
   const int* cu_c;
   const float2* stats;  // per output row: {-lse * log2(e) + kPExp, -delta}
-  uint4* xstats;        // the same as what the KV pass puts into B's extra columns
+  uint4* xstats;        // the same as what the KV pass puts into B's extra columns; float16: with the code
+                        // (mag_code) of |dO| in the last column, whose unit is 0
+  int4* range;          // float16: the codes of a tile's largest |dO|, |delta| (x, y: at the tile's first row of the
+                        // query head) and |v| (z: of the key head); at a sequence's first row, see
+                        // range_by_sequence, all its tiles', and its context's |v| (w; a shared context's at row 0)
   float none;           // KV: -lse, as the columns hold it, of a row that is not there: P = 0
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
@@ -119,7 +133,8 @@ struct BwdCfg {
   static constexpr int TMA_WARP = EW_WARPS;
   static constexpr int MMA_WARP = EW_WARPS + 1;
   static constexpr int EXT_WARP = EW_WARPS + 2;
-  static constexpr int THREADS = 32 * (EW_WARPS + (KV ? 3 : 2));
+  static constexpr int POWER_WARP = EW_WARPS + 3;  // (float16; registers are given to four warps at a time)
+  static constexpr int THREADS = 32 * (EW_WARPS + (KV ? 4 : 2));
   static constexpr int NC = BN / EW_GROUPS;  // score columns per element-wise warp
   static constexpr int TM_S = 0, TM_DP = BN, TM_P = SEP_P ? 2 * BN : 0;
   static constexpr int TM_ACC1 = (DB ? 3 : 2) * BN + (SEP_P ? BN / 2 : 0), TM_ACC2 = TM_ACC1 + (KV ? DV : 0);
@@ -135,7 +150,7 @@ struct BwdCfg {
   static constexpr int EXACT_KEYS = 64;  // Q: items of several tiles with at most so many keys sum delta themselves
   static constexpr int FEW_TERMS = 128, FEW_ROWS = 8;  // items whose P and dS keep a second part (see above)
   static constexpr int RING = 4;
-  static constexpr int ITEM_BYTES = 96;
+  static constexpr int ITEM_BYTES = 104;
   static constexpr int SMEM_BYTES = SMEM_TILES + 512 + RING * ITEM_BYTES + SUM_BYTES + 1024;
 };
 
@@ -151,10 +166,12 @@ struct BwdItem {
   int stat_h;                  // KV: stats rows of one streamed head
   int pre;                     // Q: tiles walked first for delta alone (0 or all of them)
   int few;                     // few terms or few rows: P and dS keep a second 16-bit part
+  int seq;                     // sequence, or context entry
+  float ds_mul;                // KV, float16: what takes P (dP - delta) to the dS that is held
   long long out_row;           // output row of the tile's row 0 (also its stats row in the Q pass)
   long long stat0;             // KV: stats row of (head h0, streamed row 0)
 };
-static_assert(sizeof(BwdItem) <= 96, "item ring slot");
+static_assert(sizeof(BwdItem) <= 104, "item ring slot");
 
 // The sequence that owns tile slot v when sequence b's tiles start at slot
 // cu[b] / 128 + b (strictly increasing, and at least ceil(len / 128) apart, so
@@ -171,6 +188,93 @@ __device__ __forceinline__ int find_slot_owner(const int* __restrict__ cu, int n
     hi = min(hi, lo + step);
   }
   return lo;
+}
+
+// Magnitudes as small whole numbers: 64 + X where the value is below 2^X (and
+// not below 2^(X - 2)), 0 of a 0, at most 126 (infinities).
+__device__ __forceinline__ int mag_code(float x) {  // x >= 0
+  return x > 0.f ? min(max(((__float_as_int(x) >> 23) & 255) - 126 + 64, 1), 126) : 0;
+}
+__device__ __forceinline__ int mag_code_of_square(float x) {
+  return x > 0.f ? min(max(((((__float_as_int(x) >> 23) & 255) - 125) >> 1) + 64, 1), 126) : 0;
+}
+// The power of two for dS = P (dP - delta) from the codes of |dO|, |v| and |delta|:
+// |dS| 2^power <= 2^15, half of what float16 holds.
+__device__ __forceinline__ int ds_power(int g, int v, int d) {
+  const int bound = max(g > 0 && v > 0 ? g + v - 64 : 0, d) - 64 + 1;
+  return min(max(15 - bound, -60), 60);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }  // x = 2^e
+
+// Rows [s0, s1) of sequence b in a packed batch.
+__device__ __forceinline__ void packed_rows(const BwdParams& p, int b, int& s0, int& s1) {
+  s0 = min(max(__ldg(p.cu_q + b), 0), p.T);
+  s1 = min(max(__ldg(p.cu_q + b + 1), 0), p.T);
+}
+
+// Items that see several sequences, or short ones next to a context, would read
+// many tiles' codes: another kernel gathers each sequence's at its first row.
+// (64 sequences of 32 to 256 tokens, each seeing the earlier ones and a context:
+// Q 417 -> 406, KV 625 -> 620 us.)
+__host__ __device__ __forceinline__ bool range_by_sequence(const BwdParams& p) { return p.C > 0 || p.causal; }
+
+// First row of a head's sequence b (in the order of the output, or of k), whose
+// every 128th row has its tile's codes in p.range; n: the sequence's rows.
+__device__ __forceinline__ long long range_row(const BwdParams& p, int heads, int head, int b, int& n) {
+  if (p.layout == FMLM_BWD_PACKED) {
+    int s0, s1;
+    packed_rows(p, b, s0, s1);
+    n = s1 - s0;
+    return (long long)head * p.T + s0;
+  }
+  n = p.N;
+  if (p.layout == FMLM_BWD_PADDED) n = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
+  return ((long long)b * heads + head) * p.N;
+}
+
+// Calls f for the codes of sequences [b0, b1) and heads [h0, h0 + hn) of `heads`.
+template <class F>
+__device__ __forceinline__ void for_tiles(const BwdParams& p, int heads, int h0, int hn, int b0, int b1, int lane, F f) {
+  const bool whole = range_by_sequence(p);
+  int n;
+  const long long r0 = range_row(p, heads, h0, b0, n);
+  const int k = whole ? b1 - b0 : (n + 127) >> 7;  // of each head (else b1 = b0 + 1: the sequence's tiles)
+  for (int i = lane; i < k * hn; i += 32) {
+    const int h = hn == 1 ? 0 : i / k, j = i - h * k;
+    long long r = r0 + (long long)h * (p.layout == FMLM_BWD_PACKED ? p.T : p.N) + j * 128;
+    if (whole) r = range_row(p, heads, h0 + h, b0 + j, n);
+    if (n > 0) f(p.range + r);
+  }
+}
+
+// The code of the largest |v| of the context that sequence (or entry) s sees.
+__device__ __forceinline__ int context_value_code(const BwdParams& p, int hk, int s) {
+  int n = 1;
+  const long long r = p.C == 1 ? (long long)hk * p.T : range_row(p, p.HK, hk, s, n);
+  return n > 0 ? __ldg(&p.range[r].w) : 0;
+}
+
+// KV: dS's power of two for an item, by the whole warp.
+__device__ __forceinline__ int kv_item_power(const BwdParams& p, const BwdItem& it, int lane) {
+  const bool ctx = it.a_map != 0, all = ctx && p.C == 1;
+  int g = 0, v = 0, d = 0;
+  if (ctx) v = context_value_code(p, it.a_h, it.seq);
+  else for_tiles(p, p.HK, it.a_h, 1, it.seq, it.seq + 1, lane, [&](const int4* x) { v = max(v, __ldg(&x->z)); });
+  // the rows that stream past
+  for_tiles(p, p.H, it.h0, it.heads, all ? 0 : it.seq, all || (!ctx && p.causal) ? p.B : it.seq + 1, lane, [&](const int4* x) {
+    const int2 c = __ldg(reinterpret_cast<const int2*>(x));
+    g = max(g, c.x);
+    d = max(d, c.y);
+  });
+  return ds_power(__reduce_max_sync(0xffffffffu, g), __reduce_max_sync(0xffffffffu, v), __reduce_max_sync(0xffffffffu, d));
+}
+
+// Q: the code of the largest |v| that an item's rows see, by the whole warp.
+__device__ __forceinline__ int q_item_value_code(const BwdParams& p, const BwdItem& it, int lane) {
+  int v = p.C > 0 ? context_value_code(p, it.h0, it.seq) : 0;
+  for_tiles(p, p.HK, it.h0, 1, p.causal ? 0 : it.seq, it.seq + 1, lane, [&](const int4* x) { v = max(v, __ldg(&x->z)); });
+  return __reduce_max_sync(0xffffffffu, v);
 }
 
 template <class C>
@@ -204,7 +308,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   it.stat0 = 0;
   int tile = 0;  // of its sequence
   if (ctx) {
-    const int c = find_slot_owner(p.cu_c, p.C, v, lane);
+    const int c = it.seq = find_slot_owner(p.cu_c, p.C, v, lane);
     const int c0 = min(max(__ldg(p.cu_c + c), 0), p.Tc), c1 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
     const int t = tile = v - ((c0 >> 7) + c);
     it.a_row = c0 + t * 128;
@@ -215,8 +319,9 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
     it.end0 = min(max(__ldg(p.cu_q + e), 0), p.T);
     it.stat_h = p.T;
   } else if (packed) {
-    const int b = find_slot_owner(p.cu_q, p.B, v, lane);
-    const int s0 = min(max(__ldg(p.cu_q + b), 0), p.T), s1 = min(max(__ldg(p.cu_q + b + 1), 0), p.T);
+    const int b = it.seq = find_slot_owner(p.cu_q, p.B, v, lane);
+    int s0, s1;
+    packed_rows(p, b, s0, s1);
     const int t = tile = v - ((s0 >> 7) + b);
     it.a_row = s0 + t * 128;
     it.valid = it.limit = min(max(s1 - it.a_row, 0), t >= 0 ? 128 : 0);
@@ -241,6 +346,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
     const int b = v / per_seq, t = v % per_seq;
     int L = p.N;
     if (p.layout == FMLM_BWD_PADDED) L = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
+    it.seq = b;
     tile = t;
     it.a_row = t * 128;
     it.a_b = it.b = b;
@@ -255,6 +361,7 @@ __device__ __forceinline__ BwdItem decode_bwd_item(const BwdParams& p, int w, in
   it.nt0 = tiles(it.row0, it.end0);
   if (it.valid == 0) it.nt0 = it.nt1 = 0;
   it.pre = 0;
+  it.ds_mul = 0.f;
   const int n = it.nt0 + it.nt1, terms = max(it.end0 - it.row0, 0) + max(it.end1 - it.row1, 0);
   it.few = (it.valid <= C::FEW_ROWS && tile == 0) || (long long)it.heads * terms <= C::FEW_TERMS;
   if constexpr (!C::KV) {
@@ -277,6 +384,7 @@ struct __align__(8) BwdBarriers {
   uint64_t sum_full;          // Q: every warp's part of delta is in shared memory
   uint64_t acc_full, acc_empty;
   uint64_t item_full[4], item_empty[4];
+  uint64_t mul_full[4];       // KV, float16: extra-column warp -> element-wise: the item's ds_mul
   int item_idx[4];
   uint32_t tmem_base;
   int abort_flag;
@@ -481,7 +589,8 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       mbar_init(&bar->b1_empty[i], 1);
       mbar_init(&bar->b2_empty[i], 1);
       mbar_init(&bar->item_full[i], 1);
-      mbar_init(&bar->item_empty[i], C::EW_WARPS + (KV ? 2 : 1));
+      mbar_init(&bar->mul_full[i], 1);
+      mbar_init(&bar->item_empty[i], C::EW_WARPS + (!KV ? 1 : BF16 ? 2 : 3));
     }
     mbar_init(&bar->s_full, 1);
     mbar_init(&bar->a_tm, C::EW_WARPS);
@@ -678,6 +787,22 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       }
       if (failed) break;
     }
+  } else if (KV && warp == C::POWER_WARP) {
+    // ------------------------------------------------------------ float16: dS's power of two
+    // (A warp for it, since its loads take as long as a short item: moved out of
+    // the warp above, 64 packed sequences with contexts 627 -> 608 us.)
+    if constexpr (KV && !BF16) {
+      for (uint32_t ring = 0;; ++ring) {
+        const BwdItem* slot = take_item(ring);
+        if (!slot) break;
+        const float m = BwdScale<BF16>::kInv * pow2(slot->nt0 > 0 ? kv_item_power(p, *slot, lane) : 0);
+        if (lane == 0) {
+          ring_items[ring & 3].ds_mul = m;
+          mbar_arrive(&bar->mul_full[ring & 3]);
+        }
+        release_item(ring);
+      }
+    }
   } else if (warp == C::MMA_WARP) {
     // ------------------------------------------------------------ MMA issuer
     constexpr uint32_t fmt = BF16 ? 1u : 0u;
@@ -871,7 +996,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint32_t tDP0 = tmem_base + lane_off + C::TM_DP + g * NC;
     const uint32_t tP = C::SEP_P ? tmem_base + lane_off + C::TM_P + g * (NC / 2) : tS;
     constexpr float kInv = BwdScale<BF16>::kInv;
-    const F2 sl2_2 = f2(p.scale_log2, p.scale_log2), kinv_2 = f2(kInv, kInv);
+    const F2 sl2_2 = f2(p.scale_log2, p.scale_log2);
     uint32_t ph = 0, ph2 = 0, acc_ph = 0, aload = 0, sums = 0;  // ph2: of a barrier that every other tile uses (DB)
     auto next_tile = [&]() {
       ph2 ^= ph;
@@ -947,8 +1072,15 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int nt0 = it->nt0, pre = KV ? 0 : it->pre, n = it->heads * nt0 + it->nt1 + pre;
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
+      // dS is held times 2^power (float16), over P's factor
+      float ds_mul = kInv;
+      if constexpr (!KV && !BF16) {
+        const int code = row < it->valid ? reinterpret_cast<const unsigned short*>(p.xstats + it->out_row + row)[7] : 0;
+        if (n > 0) ds_mul *= pow2(ds_power(code, q_item_value_code(p, *it, lane), mag_code(fabsf(rs.y))));
+      }
+      const F2 mul_2 = f2(ds_mul, ds_mul);
       const F2 nl_2 = f2(rs.x, rs.x);
-      F2 nd_2 = f2(rs.y * kInv, rs.y * kInv);
+      F2 nd_2 = f2(rs.y * ds_mul, rs.y * ds_mul);
       // (The first tile apart, so that the waiting results leave their registers
       // there; and apart the items of few terms, of which some sum delta themselves.)
       auto tile = [&](auto first, auto few, int i) -> bool {
@@ -985,6 +1117,12 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
             give(tP, pk, h, bar->p_full);
           }
         }
+        if constexpr (KV && !BF16) {  // (here, with few registers in use; at dS, where it spills: 608 -> 617 us)
+          if (i == 0 && !wait(&bar->mul_full[ring & 3], (ring >> 2) & 1u)) return false;
+          const float m = it->ds_mul;
+#pragma unroll
+          for (int c = 0; c < NC / 2; ++c) pr[c] = mul2(pr[c], f2(m, m));
+        }
         if constexpr (!KV) {
           const int j = kFew && i >= pre ? i - pre : i;
           const int valid = (j >= nt0 ? it->end1 - (it->row1 + (j - nt0) * BN) : it->end0 - (it->row0 + j * BN)) - g * NC;
@@ -1016,10 +1154,18 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
               if (!wait(&bar->sum_full, sums & 1u)) return false;
               ++sums;
               const float nd = -((part[0] + part[C::BM]) + (part[2 * C::BM] + part[3 * C::BM])) * kInv;
-              nd_2 = f2(nd * kInv, nd * kInv);
-              if (g == 0 && row < it->valid) {
-                const uint4 e = ext_columns<BF16>(0.f, nd);
-                *reinterpret_cast<uint2*>(&p.xstats[it->out_row + row].z) = make_uint2(e.z, e.w);
+              nd_2 = f2(nd * ds_mul, nd * ds_mul);
+              if (g == 0) {
+                if (row < it->valid) {
+                  const uint4 e = ext_columns<BF16>(0.f, nd);
+                  uint4* dst = p.xstats + it->out_row + row;
+                  dst->z = e.z;
+                  reinterpret_cast<unsigned short*>(dst)[6] = (unsigned short)e.w;
+                }
+                  if constexpr (!BF16) {
+                  const int d = __reduce_max_sync(0xffffffffu, row < it->valid ? mag_code(fabsf(nd)) : 0);
+                  if (lane == 0) atomicMax(&p.range[it->out_row].y, d);
+                }
               }
             }
             if (i < pre) {
@@ -1034,8 +1180,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
 #pragma unroll
           for (int c = h * HC; c < (h + 1) * HC; ++c) {
             F2 d = f2u(x[2 * c], x[2 * c + 1]);
-            if constexpr (!KV) d = fma2(d, kinv_2, nd_2);
-            else if constexpr (!BF16) d = mul2(d, kinv_2);
+            if constexpr (!KV) d = fma2(d, mul_2, nd_2);
             d = mul2(pr[c], d);
             pk[c] = pack2<BF16>(d);
             if constexpr (kFew) pk2[c] = pack_rest<BF16>(d, pk[c]);
@@ -1073,7 +1218,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         tc_fence_after();
         if (part * COLS < C::DV) {
           const uint32_t tO = tmem_base + lane_off + (is_dv ? C::TM_ACC1 : C::TM_ACC2) + part * COLS;
-          const float fs = is_dv ? kInv : p.scale;
+          const float fs = is_dv ? kInv : BF16 ? p.scale : p.scale * kInv * inv_pow2(KV ? it->ds_mul : ds_mul);
           const F2 f = f2(fs, fs);
 #pragma unroll
           for (int c0 = 0; c0 < COLS; c0 += 16) {
@@ -1111,45 +1256,183 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   }
 }
 
-// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}, in float32 and as
-// the KV pass's extra columns; also zeroes the item counters of the two passes that follow.  Reads O and dO
-// once (bound by HBM).  delta uses the 16-bit O that the forward pass returned:
-// its rounding (half a step per element) enters dS as |dO| * 2^-9 noise, below
-// that of dS's own rounding to 16 bits.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const uint4* __restrict__ out,
-                                                             const uint4* __restrict__ dout,
-                                                             const float* __restrict__ lse, long long rows,
-                                                             float ext_mul, float2* __restrict__ stats,
-                                                             uint4* __restrict__ xstats, int* counters) {
-  constexpr int LANES = D / 8;  // 16-byte vectors per row
-  if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long r = i / LANES;
-  float s = 0.f;
-  if (r < rows) {
-    const uint4 a = __ldg(out + i), b = __ldg(dout + i);
-    const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float2 x, y;
-      if constexpr (BF16) {
-        x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&av[e]));
-        y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&bv[e]));
-      } else {
-        x = __half22float2(*reinterpret_cast<const __half2*>(&av[e]));
-        y = __half22float2(*reinterpret_cast<const __half2*>(&bv[e]));
-      }
-      s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
-    }
-  }
+struct BwdRows {  // v, or the context's: [batch][heads][rows][D] in strides of elements
+  const uint16_t* data;
+  long long batch, head, row;
+};
+
+// Sum over the LANES neighbouring threads that share a row.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float s) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (r < rows && threadIdx.x % LANES == 0) {
-    const float nl = fmaf(-1.4426950408889634f, __ldg(lse + r), BwdScale<BF16>::kPExp);
-    stats[r] = make_float2(nl, -s);
-    xstats[r] = ext_columns<BF16>(nl * ext_mul, -s);
+  return s;
+}
+
+// a . b over a vector of eight 16-bit numbers
+template <bool BF16>
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
+  const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float x0, x1, y0, y1;
+    unf2(unpack2<BF16>(av[e]), x0, x1);
+    unf2(unpack2<BF16>(bv[e]), y0, y1);
+    s = fmaf(x0, y0, fmaf(x1, y1, s));
   }
+  return s;
+}
+
+// The code of the largest norm among `rows` rows (at most 128) from src on, by
+// the whole block; `code` is shared and was zeroed.
+template <int D, int THREADS>
+__device__ __forceinline__ int largest_norm_code(const uint16_t* src, long long stride, int rows, int* code) {
+  constexpr int LANES = D / 8, STEP = THREADS / LANES;
+  src += (threadIdx.x % LANES) * 8;
+  float m = 0.f;
+#pragma unroll
+  for (int r = threadIdx.x / LANES; r < 128; r += STEP) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < rows) x = __ldg(reinterpret_cast<const uint4*>(src + r * stride));
+    m = fmaxf(m, row_sum<LANES>(dot8<false>(x, x)));
+  }
+  const int c = __reduce_max_sync(0xffffffffu, mag_code_of_square(m));
+  if ((threadIdx.x & 31) == 0) atomicMax(code, c);
+  __syncthreads();
+  return *code;
+}
+
+// Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}, in float32 and as
+// the KV pass's extra columns; also zeroes the item counters of the two passes
+// that follow.  A block takes the rows of one 128-row tile, and reads O and dO
+// once (bound by HBM).  delta uses the 16-bit O that the forward pass returned
+// (what that costs: at the head of this file).  float16: also the rows' codes of
+// |dO| and the tile's largest; the blocks behind do the same for v's tiles.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const BwdParams p, const uint4* __restrict__ out,
+                                                             const uint4* __restrict__ dout,
+                                                             const float* __restrict__ lse, float ext_mul, const BwdRows v) {
+  constexpr int LANES = D / 8, STEP = 256 / LANES;
+  __shared__ int code[2];
+  const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x < 2) p.counter[threadIdx.x] = 0;
+  if constexpr (!BF16) {
+    if (threadIdx.x < 2) code[threadIdx.x] = 0;
+    __syncthreads();
+  }
+  unsigned i = blockIdx.x;
+  const unsigned nq = (unsigned)p.H * p.slots;
+  const bool is_v = !BF16 && i >= nq;
+  if (is_v) i -= nq;
+  const int heads = is_v ? p.HK : p.H, h = i / p.slots, slot = i % p.slots;
+  int b = 0, r0, rows;  // batch coordinate, first row, rows from there on
+  long long first;      // the first row in the order of the output (or of k)
+  if (p.layout == FMLM_BWD_PACKED) {
+    const int s = find_slot_owner(p.cu_q, p.B, slot, lane);
+    int s0, s1;
+    packed_rows(p, s, s0, s1);
+    const int t = slot - ((s0 >> 7) + s);
+    r0 = s0 + t * 128;
+    rows = t >= 0 ? s1 - r0 : 0;
+    first = (long long)h * p.T + r0;
+  } else {
+    const int per_seq = (p.N + 127) / 128;
+    b = slot / per_seq;
+    r0 = (slot % per_seq) * 128;
+    int L = p.N;
+    if (p.layout == FMLM_BWD_PADDED) L = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
+    rows = L - r0;
+    first = ((long long)b * heads + h) * p.N + r0;
+  }
+  rows = min(rows, 128);
+  if (rows <= 0) return;
+  if constexpr (!BF16) {
+    if (is_v) {
+      const int c = largest_norm_code<D, 256>(v.data + b * v.batch + h * v.head + r0 * v.row, v.row, rows, code);
+      if (threadIdx.x == 0) *reinterpret_cast<int2*>(&p.range[first].z) = make_int2(c, 0);
+      return;
+    }
+  }
+  int g_max = 0, d_max = 0;
+  const uint4 *o = out + first * LANES + threadIdx.x, *d = dout + first * LANES + threadIdx.x;
+  float2* stats = const_cast<float2*>(p.stats);
+#pragma unroll 4
+  for (int r = threadIdx.x / LANES; r < 128; r += STEP, o += 256, d += 256) {
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    float l = 0.f;
+    if (r < rows) {
+      x = __ldg(o);
+      y = __ldg(d);
+      l = __ldg(lse + first + r);
+    }
+    const float s = row_sum<LANES>(dot8<BF16>(x, y));
+    float g = 0.f;
+    if constexpr (!BF16) g = row_sum<LANES>(dot8<BF16>(y, y));
+    if (r < rows && threadIdx.x % LANES == 0) {
+      const float nl = fmaf(-1.4426950408889634f, l, BwdScale<BF16>::kPExp);
+      stats[first + r] = make_float2(nl, -s);
+      uint4 e = ext_columns<BF16>(nl * ext_mul, -s);
+      if constexpr (!BF16) {
+        const int c = mag_code_of_square(g);
+        e.w |= (uint32_t)c << 16;
+        g_max = max(g_max, c);
+        d_max = max(d_max, mag_code(fabsf(s)));
+      }
+      p.xstats[first + r] = e;
+    }
+  }
+  if constexpr (!BF16) {
+    g_max = __reduce_max_sync(0xffffffffu, g_max);
+    d_max = __reduce_max_sync(0xffffffffu, d_max);
+    if (lane == 0) {
+      atomicMax(&code[0], g_max);
+      atomicMax(&code[1], d_max);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *reinterpret_cast<int2*>(&p.range[first].x) = make_int2(code[0], code[1]);
+  }
+}
+
+// float16, packed: what range_by_sequence needs.  The first blocks find the code
+// of the largest |v| of each context, 128 rows of an entry each, and leave it at
+// the sequence that sees it (a shared context's at the head's first row; the
+// kernel before zeroed it).  The others gather the tiles' codes of a sequence and
+// head, a warp each.  Maxima of whole numbers do not depend on their order.
+template <int D>
+__global__ void __launch_bounds__(128) attn_bwd_range_kernel(const BwdParams p, const BwdRows vc, int context_blocks) {
+  const int lane = threadIdx.x & 31;
+  if ((int)blockIdx.x < context_blocks) {
+    __shared__ int code;
+    if (threadIdx.x == 0) code = 0;
+    __syncthreads();
+    const int h = blockIdx.x / p.cslots, slot = blockIdx.x % p.cslots;
+    const int c = find_slot_owner(p.cu_c, p.C, slot, lane);
+    const int c0 = min(max(__ldg(p.cu_c + c), 0), p.Tc), c1 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
+    const int t = slot - ((c0 >> 7) + c), r0 = c0 + t * 128, rows = t >= 0 ? min(c1 - r0, 128) : 0;
+    int q0 = 0, q1 = 1;
+    if (p.C > 1) packed_rows(p, c, q0, q1);
+    if (rows <= 0 || q1 <= q0) return;  // (an entry that no query sees)
+    const int x = largest_norm_code<D, 128>(vc.data + h * vc.head + r0 * vc.row, vc.row, rows, &code);
+    if (threadIdx.x == 0) atomicMax(&p.range[(long long)h * p.T + q0].w, x);
+    return;
+  }
+  const long long i = (long long)(blockIdx.x - context_blocks) * 4 + (threadIdx.x >> 5);  // query heads, then v's
+  const int head = (int)(i / p.B), b = (int)(i % p.B);
+  if (head >= p.H + p.HK) return;
+  const bool is_v = head >= p.H;
+  int n;
+  int4* x = p.range + range_row(p, 0, is_v ? head - p.H : head, b, n);
+  int g = 0, d = 0;  // (v: its code in g)
+  for (int t = lane * 128; t < n; t += 32 * 128) {
+    g = max(g, is_v ? x[t].z : x[t].x);
+    if (!is_v) d = max(d, x[t].y);
+  }
+  g = __reduce_max_sync(0xffffffffu, g);
+  d = __reduce_max_sync(0xffffffffu, d);
+  if (lane != 0 || n <= 128) return;
+  if (is_v) x->z = g;
+  else *reinterpret_cast<int2*>(x) = make_int2(g, d);
 }
 
 }  // namespace fmlm

@@ -332,8 +332,8 @@ def flash_attn_mlm_train(
     The arguments of ``flash_attn_mlm_fwd``; padded q/k/v with a context or
     ``causal_query_seq_attn`` are packed first (and their gradients unpacked).
     Returns out in q's layout.  Gradients flow to q, k, v, context_k and
-    context_v.  float16: as with any float16 gradient, the products of dout
-    with v must stay inside float16's range (loss scaling sees to that).
+    context_v.  float16: the gradients have to lie in float16's range (loss
+    scaling sees to that); what they are computed from need not.
 
     To capture the backward pass into a CUDA graph, call ``flash_attn_mlm_fwd``
     and ``flash_attn_mlm_bwd``, which involve no autograd graph.
