@@ -199,10 +199,13 @@ __device__ __forceinline__ int mag_code_of_square(float x) {
   return x > 0.f ? min(max(((((__float_as_int(x) >> 23) & 255) - 125) >> 1) + 64, 1), 126) : 0;
 }
 // The power of two for dS = P (dP - delta) from the codes of |dO|, |v| and |delta|:
-// |dS| 2^power <= 2^15, half of what float16 holds.
+// |dS| 2^power <= 2^15, half of what float16 holds.  But dS is made smaller only
+// for the sake of |dO|, as if |v| were 32 at most: one far larger row of v would
+// push the others' dS among the subnormals, though nothing may attend to it.
 __device__ __forceinline__ int ds_power(int g, int v, int d) {
   const int bound = max(g > 0 && v > 0 ? g + v - 64 : 0, d) - 64 + 1;
-  return min(max(15 - bound, -60), 60);
+  const int least = min(0, 15 - (g - 64 + 5 + 1));
+  return min(max(15 - bound, least), 60);
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }  // x = 2^e
@@ -642,15 +645,16 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     atomicExch(p.err, 1);
   };
   // Whole-warp wait; false once anything in the CTA has given up.
-  auto wait = [&](uint64_t* b, uint32_t ph) -> bool {
+  auto wait_for = [&](uint64_t* b, uint32_t ph, uint64_t limit) -> bool {
     if (__all_sync(0xffffffffu, mbar_try_wait(smem_u32(b), ph))) return true;
-    if (!mbar_wait(b, ph, abort_flag, tmo)) fail();
+    if (!mbar_wait(b, ph, abort_flag, limit)) fail();
     failed = __any_sync(0xffffffffu, failed);
     return !failed;
   };
+  auto wait = [&](uint64_t* b, uint32_t ph) -> bool { return wait_for(b, ph, tmo); };
   // The next published item, in its ring slot until release_item; nullptr: no more.
-  auto take_item = [&](uint32_t ring) -> const BwdItem* {
-    if (failed || !wait(&bar->item_full[ring & 3], (ring >> 2) & 1u)) return nullptr;
+  auto take_item = [&](uint32_t ring, uint64_t limit) -> const BwdItem* {
+    if (failed || !wait_for(&bar->item_full[ring & 3], (ring >> 2) & 1u, limit)) return nullptr;
     const int w = *reinterpret_cast<volatile int*>(&bar->item_idx[ring & 3]);
     return w < num_items ? ring_items + (ring & 3) : nullptr;
   };
@@ -749,7 +753,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     const uint4 none = ext_columns<BF16>(p.none, 0.f);
     uint32_t fill = 0;
     for (uint32_t ring = 0;; ++ring) {
-      const BwdItem* slot = take_item(ring);
+      const BwdItem* slot = take_item(ring, tmo);
       if (!slot) break;
       const int nt0 = slot->nt0, n = slot->heads * nt0, row0 = slot->row0, end0 = slot->end0, stat_h = slot->stat_h;
       const uint4* src = p.xstats + slot->stat0;
@@ -790,10 +794,11 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
   } else if (KV && warp == C::POWER_WARP) {
     // ------------------------------------------------------------ float16: dS's power of two
     // (A warp for it, since its loads take as long as a short item: moved out of
-    // the warp above, 64 packed sequences with contexts 627 -> 608 us.)
+    // the warp above, 64 packed sequences with contexts 627 -> 608 us.  It waits
+    // as long as the item before lasts; what hangs gives up in another warp.)
     if constexpr (KV && !BF16) {
       for (uint32_t ring = 0;; ++ring) {
-        const BwdItem* slot = take_item(ring);
+        const BwdItem* slot = take_item(ring, 1024 * tmo);
         if (!slot) break;
         const float m = BwdScale<BF16>::kInv * pow2(slot->nt0 > 0 ? kv_item_power(p, *slot, lane) : 0);
         if (lane == 0) {
@@ -893,7 +898,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
     Stage s_st, d_st, c_st;  // stages of the next S, the next dP, the current accumulations
     uint32_t aload = 0, ph = 0, ph2 = 0, acc_ph = 1;  // ph2: of a barrier that every other tile uses (DB)
     for (uint32_t ring = 0;; ++ring) {
-      const BwdItem* slot = take_item(ring);
+      const BwdItem* slot = take_item(ring, tmo);
       if (!slot) break;
       const int nt0 = slot->nt0, nt1 = slot->nt1, pre = KV ? 0 : slot->pre, n = slot->heads * nt0 + nt1 + pre;
       // valid rows of each range's last tile
@@ -1066,7 +1071,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       }
       res_dst = nullptr;
     };
-    const BwdItem* it = take_item(0);
+    const BwdItem* it = take_item(0, tmo);
     if (C::ATM && it && it->heads * it->nt0 + it->nt1 > 0 && !copy_a()) it = nullptr;
     for (uint32_t ring = 0; it; ++ring) {
       const int nt0 = it->nt0, pre = KV ? 0 : it->pre, n = it->heads * nt0 + it->nt1 + pre;
@@ -1203,7 +1208,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       // dP of the last tile was the last MMA to read the stationary tiles (and
       // came after the last S), so the next item's can move in: its first
       // scores follow this item's last accumulations at once.
-      const BwdItem* next = take_item(ring + 1);
+      const BwdItem* next = take_item(ring + 1, tmo);
       if (failed) break;
       const int next_n = next ? next->heads * next->nt0 + next->nt1 : 0;
       if (C::ATM && next_n > 0 && !copy_a()) break;

@@ -303,3 +303,20 @@ def test_float16_zero_gradients_and_values():
         assert not got["dq"].any() and not got["dk"].any()
         assert bool(got["dv"].any()) == bool(b.any())
     fm().check_device_errors(device())
+
+
+@pytest.mark.parametrize("n", [100, 512, 3000])
+@pytest.mark.parametrize("size", [1.0, 1e-2])
+def test_float16_large_values_that_nothing_attends_to(n, size):
+    """One row of v near float16's end whose key no query takes (scores of -100): the gradients of the others
+    are as near as without it (dS of size 1, of 1e-2 over so few keys, is in float16's normal range as it is)."""
+    g = torch.Generator().manual_seed(15)
+    q, k, v, do = (torch.randn((1, 1, n, 64), generator=g) for _ in range(4))
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[0, 0, 7, 0], v[0, 0, 7] = -200.0, 60000.0 * torch.sign(v[0, 0, 7])
+    q, k, v, do = (x.to(F16).to(DEV) for x in (q, k, v, do * size))
+    got = gradients(q, k, v, do, 0.125)
+    fm().check_device_errors(device())
+    ratios = against_once_rounded(*(x[0, 0] for x in (q, k, v, do)), 0.125, [got[x][0, 0] for x in ("dq", "dk", "dv")])
+    # (1e-2 over 3000 keys: dS of 1e-2 / 3000 lies 2 bits below the normal range, where a step is 4 times as large)
+    assert max(ratios) <= (4 * ONCE if n == 3000 and size < 1 else ONCE), ratios
