@@ -29,7 +29,8 @@
 // only rounded at the end), but not over a few, where O is as large as v: two
 // keys, 2.4.  So a Q item whose keys fit one tile (or are at most 64 in two
 // ranges, which it then walks twice) sums delta = sum_k P dP itself, in 32 bits
-// (1.4), and leaves it for the KV pass, which runs after.
+// (1.4), and leaves it for the KV pass, which runs after.  Rows of many keys
+// whose probability lies on a few keep O's rounding (2.2 at scores of deviation 3).
 //
 // P and dS are rounded to 16 bits for the tensor cores, half a step of each
 // term: next to the rounding of the result that is a factor of 1.4 in a
@@ -42,17 +43,17 @@
 // float16 P is held times 2^12 (P <= 1), and dS times a power of two that brings
 // its bound |dO| |v| + |delta| to 2^15: as it is, dS of long rows or of small dO
 // would lie among float16's subnormals (4096 keys, dO of 1e-3: dq and dk 8 times
-// as far off as gradients rounded once, now 1.4), and dS of large dO past its
+// as far off as gradients rounded once, now 1.1), and dS of large dO past its
 // end.  A Q item's rows have each their own power, from the row's dO and the
 // largest v that it sees; a KV item one, from its sequence's v and the dO and
 // delta that stream past.  The statistics kernel leaves each tile's largest, so
 // that none depends on rows it does not see.
 //
 // What bounds it: the tensor pipe at head_dim 128 (16 heads of 8192 tokens,
-// bf16: Q pass 629 us, 1310 TFLOP/s; KV pass 728 us, 1511 TFLOP/s, 71 % of the
+// bf16: Q pass 629 us, 1310 TFLOP/s; KV pass 728 us, 1511 TFLOP/s, 70 % of the
 // tensor cycles), the chain exponentials - TMEM - MMA at head_dim 64 (2 x 16
-// heads of 2048 tokens: 75 and 88 us, tensor pipe 39 and 53 %, exponentials'
-// unit 52 and 47 %).
+// heads of 2048 tokens: 76 and 90 us, tensor pipe 40 and 52 %, exponentials'
+// unit 53 and 46 %).
 //
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),

@@ -226,7 +226,8 @@ def qk_norm_rope(
     transposed among them.
 
     ``normalize``: x / sqrt(mean(x^2) + eps) over the head dimension, times
-    ``q_weight`` / ``k_weight`` [D] (float32 or q's dtype; None: ones).
+    ``q_weight`` / ``k_weight`` [D] (float32 or q's dtype; None: ones).  The
+    squares are summed in float32 (a bfloat16 row longer than 2^64 overflows it).
     ``rotary`` (None: no rotation): the token's index in its sequence is its
     position, plus ``position_offsets[b]`` (int32 [B]: tokens that came before,
     as a cached context's), or ``positions`` (int32 [B, N], packed [T]) gives
