@@ -64,10 +64,15 @@ int encode_maps(CUtensorMap* m, const fmlm_attn_bwd_args* a, bool ctx, int qrows
 template <int D, bool BF16>
 int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, cudaStream_t s) {
   using C = BwdCfg<D, false>;
-  // A block for every tile of every head; float16: and of v's heads, and of the context's.
-  const long long blocks = (long long)(BF16 ? p.H : p.H + p.HK) * p.slots, cblocks = (long long)p.HK * p.cslots;
-  const long long rblocks = cblocks + ((long long)(p.H + p.HK) * p.B + 3) / 4;
-  if (blocks > 0x7fffffffLL || (!BF16 && rblocks > 0x7fffffffLL)) return set_error(FMLM_ERR_INVALID, "problem too large");
+  // Tile slots of the statistics (float16: of v's heads too) and of the context's
+  // v; a block takes several where they are many and short.
+  const long long slots = (long long)(BF16 ? p.H : p.H + p.HK) * p.slots, cslots = (long long)p.HK * p.cslots;
+  const long long many = (long long)device_sm_count() * 16;
+  const bool packed = a->layout == FMLM_BWD_PACKED;
+  const bool short_q = slots >= many && (packed ? p.T / p.slots : std::min(p.N, 128)) <= 32;
+  const bool short_c = cslots >= many && p.Tc / p.cslots <= 32;
+  const long long gather = ((long long)(p.H + p.HK) * p.B + 3) / 4;
+  if (slots > 0x7fffffffLL || cslots + gather > 0x7fffffffLL) return set_error(FMLM_ERR_INVALID, "problem too large");
   // Every map before the first launch: a refused view leaves nothing half done.
   const bool ctx = p.C > 0;
   CUtensorMap m[12];
@@ -77,12 +82,23 @@ int run_bwd(const fmlm_attn_bwd_args* a, const BwdParams& p, float ext_mul, cuda
   auto lay = [](const fmlm_view4& v) {
     return BwdRows{reinterpret_cast<const uint16_t*>(v.data), v.batch_stride, v.head_stride, v.row_stride};
   };
-  attn_bwd_stats_kernel<D, BF16><<<(unsigned)blocks, 256, 0, s>>>(
-      p, reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, ext_mul, lay(a->v));
+  auto stats = [&](auto per_block) {
+    constexpr int K = decltype(per_block)::value;
+    attn_bwd_stats_kernel<D, BF16, K><<<(unsigned)((slots + K - 1) / K), 256, 0, s>>>(
+        p, reinterpret_cast<const uint4*>(a->out), reinterpret_cast<const uint4*>(a->dout.data), a->lse, ext_mul, lay(a->v));
+  };
+  if (short_q) stats(std::integral_constant<int, 8>());
+  else stats(std::integral_constant<int, 1>());
   rc = check_launch("attn_bwd_stats_kernel");
   if constexpr (!BF16) {
     if (!rc && range_by_sequence(p)) {
-      attn_bwd_range_kernel<D><<<(unsigned)rblocks, 128, 0, s>>>(p, lay(a->v_context), (int)cblocks);
+      auto range = [&](auto per_block) {
+        constexpr int K = decltype(per_block)::value;
+        const long long cblocks = (cslots + K - 1) / K;
+        attn_bwd_range_kernel<D, K><<<(unsigned)(cblocks + gather), 128, 0, s>>>(p, lay(a->v_context), (int)cblocks);
+      };
+      if (short_c) range(std::integral_constant<int, 4>());
+      else range(std::integral_constant<int, 1>());
       rc = check_launch("attn_bwd_range_kernel");
     }
   }

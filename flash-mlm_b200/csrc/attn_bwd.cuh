@@ -85,8 +85,9 @@ struct BwdParams {
   uint4* xstats;        // the same as what the KV pass puts into B's extra columns; float16: with the code
                         // (mag_code) of |dO| in the last column, whose unit is 0
   int4* range;          // float16: the codes of a tile's largest |dO|, |delta| (x, y: at the tile's first row of the
-                        // query head) and |v| (z: of the key head); at a sequence's first row, see
-                        // range_by_sequence, all its tiles', and its context's |v| (w; a shared context's at row 0)
+                        // query head) and |v| (z: of the key head); at a sequence's first row, where
+                        // range_by_sequence, all its tiles' (and in z, times 256, that of all sequences up to it)
+                        // and its context's |v| (w; a shared context's at row 0)
   float none;           // KV: -lse, as the columns hold it, of a row that is not there: P = 0
   int* counter;
   void *dq, *dk, *dv, *dkc, *dvc;
@@ -217,67 +218,63 @@ __device__ __forceinline__ void packed_rows(const BwdParams& p, int b, int& s0, 
   s1 = min(max(__ldg(p.cu_q + b + 1), 0), p.T);
 }
 
-// Items that see several sequences, or short ones next to a context, would read
-// many tiles' codes: another kernel gathers each sequence's at its first row.
-// (64 sequences of 32 to 256 tokens, each seeing the earlier ones and a context:
-// Q 417 -> 406, KV 625 -> 620 us.)
+// Items that see several sequences would read many tiles' codes: another kernel
+// gathers each sequence's at its first row (64 sequences of 32 to 256 tokens, each
+// seeing the earlier ones and a context: Q 417 -> 406, KV 625 -> 620 us).
 __host__ __device__ __forceinline__ bool range_by_sequence(const BwdParams& p) { return p.C > 0 || p.causal; }
 
-// First row of a head's sequence b (in the order of the output, or of k), whose
-// every 128th row has its tile's codes in p.range; n: the sequence's rows.
-__device__ __forceinline__ long long range_row(const BwdParams& p, int heads, int head, int b, int& n) {
-  if (p.layout == FMLM_BWD_PACKED) {
-    int s0, s1;
-    packed_rows(p, b, s0, s1);
-    n = s1 - s0;
-    return (long long)head * p.T + s0;
-  }
-  n = p.N;
-  if (p.layout == FMLM_BWD_PADDED) n = min(max(__ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b), 0), p.N);
-  return ((long long)b * heads + head) * p.N;
+// KV: whether the rows that stream past are of several sequences.
+__device__ __forceinline__ bool streams_several(const BwdParams& p, const BwdItem& it) {
+  return it.a_map ? p.C == 1 : p.causal != 0;
 }
 
-// Calls f for the codes of sequences [b0, b1) and heads [h0, h0 + hn) of `heads`.
-template <class F>
-__device__ __forceinline__ void for_tiles(const BwdParams& p, int heads, int h0, int hn, int b0, int b1, int lane, F f) {
-  const bool whole = range_by_sequence(p);
-  int n;
-  const long long r0 = range_row(p, heads, h0, b0, n);
-  const int k = whole ? b1 - b0 : (n + 127) >> 7;  // of each head (else b1 = b0 + 1: the sequence's tiles)
-  for (int i = lane; i < k * hn; i += 32) {
-    const int h = hn == 1 ? 0 : i / k, j = i - h * k;
-    long long r = r0 + (long long)h * (p.layout == FMLM_BWD_PACKED ? p.T : p.N) + j * 128;
-    if (whole) r = range_row(p, heads, h0 + h, b0 + j, n);
-    if (n > 0) f(p.range + r);
-  }
-}
-
-// The code of the largest |v| of the context that sequence (or entry) s sees.
-__device__ __forceinline__ int context_value_code(const BwdParams& p, int hk, int s) {
-  int n = 1;
-  const long long r = p.C == 1 ? (long long)hk * p.T : range_row(p, p.HK, hk, s, n);
-  return n > 0 ? __ldg(&p.range[r].w) : 0;
+// KV: the code of the largest |v| of an item's keys (a context's: of its entry).
+__device__ __forceinline__ int kv_item_value_code(const BwdParams& p, const BwdItem& it) {
+  if (it.a_map) return __ldg(&p.range[(long long)it.a_h * p.T + (p.C == 1 ? 0 : it.row0)].w);
+  return __ldg(&p.range[it.out_row].z) & 255;
 }
 
 // KV: dS's power of two for an item, by the whole warp.
-__device__ __forceinline__ int kv_item_power(const BwdParams& p, const BwdItem& it, int lane) {
-  const bool ctx = it.a_map != 0, all = ctx && p.C == 1;
-  int g = 0, v = 0, d = 0;
-  if (ctx) v = context_value_code(p, it.a_h, it.seq);
-  else for_tiles(p, p.HK, it.a_h, 1, it.seq, it.seq + 1, lane, [&](const int4* x) { v = max(v, __ldg(&x->z)); });
-  // the rows that stream past
-  for_tiles(p, p.H, it.h0, it.heads, all ? 0 : it.seq, all || (!ctx && p.causal) ? p.B : it.seq + 1, lane, [&](const int4* x) {
+__device__ __forceinline__ int kv_item_power(const BwdParams& p, const BwdItem& it, bool several, int lane) {
+  const int v = kv_item_value_code(p, it), heads = it.heads;
+  const int4* range = p.range + it.stat0;
+  int g = 0, d = 0;
+  auto take = [&](const int4* x) {
     const int2 c = __ldg(reinterpret_cast<const int2*>(x));
     g = max(g, c.x);
     d = max(d, c.y);
-  });
-  return ds_power(__reduce_max_sync(0xffffffffu, g), __reduce_max_sync(0xffffffffu, v), __reduce_max_sync(0xffffffffu, d));
+  };
+  if (!several) {
+    const int k = range_by_sequence(p) ? 1 : (it.end0 - it.row0 + 127) >> 7;  // a head's
+    for (int i = lane; i < k * heads; i += 32) {
+      const int h = heads == 1 ? 0 : i / k;
+      take(range + (long long)h * it.stat_h + it.row0 + (i - h * k) * 128);
+    }
+  } else {  // all sequences (of a shared context), or those from the item's on
+    const int b0 = it.a_map ? 0 : it.seq, nb = p.B - b0;
+    for (int i = lane; i < nb * heads; i += 32) {
+      const int h = heads == 1 ? 0 : i / nb;
+      int s0, s1;
+      packed_rows(p, b0 + i - h * nb, s0, s1);
+      if (s1 > s0) take(range + (long long)h * it.stat_h + s0);
+    }
+  }
+  return ds_power(__reduce_max_sync(0xffffffffu, g), v, __reduce_max_sync(0xffffffffu, d));
 }
 
 // Q: the code of the largest |v| that an item's rows see, by the whole warp.
 __device__ __forceinline__ int q_item_value_code(const BwdParams& p, const BwdItem& it, int lane) {
-  int v = p.C > 0 ? context_value_code(p, it.h0, it.seq) : 0;
-  for_tiles(p, p.HK, it.h0, 1, p.causal ? 0 : it.seq, it.seq + 1, lane, [&](const int4* x) { v = max(v, __ldg(&x->z)); });
+  const bool packed = p.layout == FMLM_BWD_PACKED;
+  const int r0 = !packed ? 0 : p.causal ? min(max(__ldg(p.cu_q + it.seq), 0), p.T) : p.C > 0 ? it.row1 : it.row0;
+  const int4* at = p.range + ((packed ? (long long)it.h0 * p.T : ((long long)it.b * p.HK + it.h0) * p.N) + r0);
+  int v = 0;
+  if (range_by_sequence(p)) {
+    const int2 c = __ldg(reinterpret_cast<const int2*>(&at->z));
+    v = p.causal ? c.x >> 8 : c.x & 255;
+    if (p.C > 0) v = max(v, p.C == 1 ? __ldg(&p.range[(long long)it.h0 * p.T].w) : c.y);
+    return v;
+  }
+  for (int t = lane * 128; t < it.end0 - r0; t += 32 * 128) v = max(v, __ldg(&at[t].z) & 255);
   return __reduce_max_sync(0xffffffffu, v);
 }
 
@@ -758,7 +755,10 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       if (!slot) break;
       const int nt0 = slot->nt0, n = slot->heads * nt0, row0 = slot->row0, end0 = slot->end0, stat_h = slot->stat_h;
       const uint4* src = p.xstats + slot->stat0;
-      release_item(ring);
+      // float16, one tile: its columns hold the codes that ds_mul is found from
+      const bool one = !BF16 && n == 1 && !streams_several(p, *slot);
+      const int v = one ? kv_item_value_code(p, *slot) : 0;
+      if (!one) release_item(ring);
       uint4 x[BN / 32];
       int t = 0;
       auto load = [&]() {  // tile t of the head at src, and on to the next
@@ -790,10 +790,30 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
         if (saturated) atomicExch(p.err, kErrStatistics);
         if (i + 1 < n) load();
       }
+      if constexpr (!BF16) {
+        if (one && !failed) {
+          int g = 0, d = 0;
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+            float d0, d1, d2, o;
+            unf2(unpack2<BF16>(x[c].z), d0, d1);
+            unf2(unpack2<BF16>(x[c].w & 0xffffu), d2, o);
+            g = max(g, (int)(x[c].w >> 16));
+            d = max(d, mag_code(fabsf(fmaf(d0, 0x1p12f, fmaf(d2, 0x1p-12f, d1)))));
+          }
+          d = __reduce_max_sync(0xffffffffu, d);
+          const int power = ds_power(__reduce_max_sync(0xffffffffu, g), v, d);
+          if (lane == 0) {
+            ring_items[ring & 3].ds_mul = BwdScale<BF16>::kInv * pow2(power);
+            mbar_arrive(&bar->mul_full[ring & 3]);
+          }
+          release_item(ring);
+        }
+      }
       if (failed) break;
     }
   } else if (KV && warp == C::POWER_WARP) {
-    // ------------------------------------------------------------ float16: dS's power of two
+    // ------------------------------------------------------------ float16: ds_mul of items of several tiles
     // (A warp for it, since its loads take as long as a short item: moved out of
     // the warp above, 64 packed sequences with contexts 627 -> 608 us.  It waits
     // as long as the item before lasts; what hangs gives up in another warp.)
@@ -801,10 +821,13 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       for (uint32_t ring = 0;; ++ring) {
         const BwdItem* slot = take_item(ring, 1024 * tmo);
         if (!slot) break;
-        const float m = BwdScale<BF16>::kInv * pow2(slot->nt0 > 0 ? kv_item_power(p, *slot, lane) : 0);
-        if (lane == 0) {
-          ring_items[ring & 3].ds_mul = m;
-          mbar_arrive(&bar->mul_full[ring & 3]);
+        const bool several = streams_several(p, *slot);
+        if (slot->heads * slot->nt0 != 1 || several) {
+          const float m = BwdScale<BF16>::kInv * pow2(slot->nt0 > 0 ? kv_item_power(p, *slot, several, lane) : 0);
+          if (lane == 0) {
+            ring_items[ring & 3].ds_mul = m;
+            mbar_arrive(&bar->mul_full[ring & 3]);
+          }
         }
         release_item(ring);
       }
@@ -1078,7 +1101,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
       const int nt0 = it->nt0, pre = KV ? 0 : it->pre, n = it->heads * nt0 + it->nt1 + pre;
       float2 rs = make_float2(0.f, 0.f);
       if (!KV && row < it->valid) rs = __ldg(p.stats + it->out_row + row);
-      // dS is held times 2^power (float16), over P's factor
+      // What takes P (dP - delta) to the dS that is held (KV, float16: it->ds_mul).
       float ds_mul = kInv;
       if constexpr (!KV && !BF16) {
         const int code = row < it->valid ? reinterpret_cast<const unsigned short*>(p.xstats + it->out_row + row)[7] : 0;
@@ -1168,7 +1191,7 @@ __global__ void __launch_bounds__(BwdCfg<D, KV>::THREADS, 1)
                   dst->z = e.z;
                   reinterpret_cast<unsigned short*>(dst)[6] = (unsigned short)e.w;
                 }
-                  if constexpr (!BF16) {
+                if constexpr (!BF16) {
                   const int d = __reduce_max_sync(0xffffffffu, row < it->valid ? mag_code(fabsf(nd)) : 0);
                   if (lane == 0) atomicMax(&p.range[it->out_row].y, d);
                 }
@@ -1290,48 +1313,51 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
   return s;
 }
 
-// The code of the largest norm among `rows` rows (at most 128) from src on, by
-// the whole block; `code` is shared and was zeroed.
+// The code of the largest norm among `rows` rows (at most 128) from src on, over
+// the lanes of a warp, by THREADS threads of which this is number t.
 template <int D, int THREADS>
-__device__ __forceinline__ int largest_norm_code(const uint16_t* src, long long stride, int rows, int* code) {
+__device__ __forceinline__ int largest_norm_code(const uint16_t* src, long long stride, int rows, int t) {
   constexpr int LANES = D / 8, STEP = THREADS / LANES;
-  src += (threadIdx.x % LANES) * 8;
+  src += (t % LANES) * 8;
   float m = 0.f;
-#pragma unroll
-  for (int r = threadIdx.x / LANES; r < 128; r += STEP) {
+#pragma unroll 8
+  for (int r0 = 0; r0 < rows; r0 += STEP) {
+    const int r = r0 + t / LANES;
     uint4 x = make_uint4(0, 0, 0, 0);
     if (r < rows) x = __ldg(reinterpret_cast<const uint4*>(src + r * stride));
     m = fmaxf(m, row_sum<LANES>(dot8<false>(x, x)));
   }
-  const int c = __reduce_max_sync(0xffffffffu, mag_code_of_square(m));
-  if ((threadIdx.x & 31) == 0) atomicMax(code, c);
-  __syncthreads();
-  return *code;
+  return __reduce_max_sync(0xffffffffu, mag_code_of_square(m));
 }
 
 // Per output row: {-lse * log2(e) + kPExp, -rowsum(dO * O)}, in float32 and as
 // the KV pass's extra columns; also zeroes the item counters of the two passes
-// that follow.  A block takes the rows of one 128-row tile, and reads O and dO
-// once (bound by HBM).  delta uses the 16-bit O that the forward pass returned
-// (what that costs: at the head of this file).  float16: also the rows' codes of
-// |dO| and the tile's largest; the blocks behind do the same for v's tiles.
-template <int D, bool BF16>
+// that follow.  Reads O and dO once (bound by HBM).  delta uses the 16-bit O that
+// the forward pass returned (what that costs: at the head of this file).
+// float16: also the rows' codes of |dO| and each tile's largest; the blocks behind
+// do the same for v's tiles.  A block takes SLOTS tile slots of 128 rows, one after the
+// other's heads: one where there are few, so that they spread over the GPU,
+// eight (a warp each) where there are many of few rows (4096 sequences of 1 to 16
+// tokens, 8 heads: 26 us, one slot a block 103; 16 sequences of 512, 32 heads of
+// 128: one slot a block 27 us, eight 52).
+template <int D, bool BF16, int SLOTS>
 __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const BwdParams p, const uint4* __restrict__ out,
                                                              const uint4* __restrict__ dout,
                                                              const float* __restrict__ lse, float ext_mul, const BwdRows v) {
-  constexpr int LANES = D / 8, STEP = 256 / LANES;
-  __shared__ int code[2];
-  const int lane = threadIdx.x & 31;
+  constexpr int THREADS = 256 / SLOTS, LANES = D / 8, STEP = THREADS / LANES;
+  __shared__ int code[2];  // (one slot: its largest)
+  const int lane = threadIdx.x & 31, tid = threadIdx.x % THREADS;
   if (blockIdx.x == 0 && threadIdx.x < 2) p.counter[threadIdx.x] = 0;
-  if constexpr (!BF16) {
+  if constexpr (!BF16 && SLOTS == 1) {
     if (threadIdx.x < 2) code[threadIdx.x] = 0;
     __syncthreads();
   }
-  unsigned i = blockIdx.x;
-  const unsigned nq = (unsigned)p.H * p.slots;
-  const bool is_v = !BF16 && i >= nq;
+  long long i = (long long)blockIdx.x * SLOTS + threadIdx.x / THREADS;
+  const long long nq = (long long)p.H * p.slots;
+  const bool is_v = i >= nq;
   if (is_v) i -= nq;
-  const int heads = is_v ? p.HK : p.H, h = i / p.slots, slot = i % p.slots;
+  if (is_v && (BF16 || i >= (long long)p.HK * p.slots)) return;
+  const int heads = is_v ? p.HK : p.H, h = (int)i / p.slots, slot = (int)i - h * p.slots;
   int b = 0, r0, rows;  // batch coordinate, first row, rows from there on
   long long first;      // the first row in the order of the output (or of k)
   if (p.layout == FMLM_BWD_PACKED) {
@@ -1353,18 +1379,29 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const BwdParams p, 
   }
   rows = min(rows, 128);
   if (rows <= 0) return;
+  // the largest over the slot's threads, valid in its thread 0
+  auto largest = [&](int c, int* shared) {
+    if constexpr (SLOTS == 1) {
+      if (lane == 0) atomicMax(shared, c);
+      __syncthreads();
+      return *shared;
+    } else {
+      return c;
+    }
+  };
   if constexpr (!BF16) {
     if (is_v) {
-      const int c = largest_norm_code<D, 256>(v.data + b * v.batch + h * v.head + r0 * v.row, v.row, rows, code);
-      if (threadIdx.x == 0) *reinterpret_cast<int2*>(&p.range[first].z) = make_int2(c, 0);
+      const int c = largest(largest_norm_code<D, THREADS>(v.data + b * v.batch + h * v.head + r0 * v.row, v.row, rows, tid), code);
+      if (tid == 0) *reinterpret_cast<int2*>(&p.range[first].z) = make_int2(c, 0);
       return;
     }
   }
   int g_max = 0, d_max = 0;
-  const uint4 *o = out + first * LANES + threadIdx.x, *d = dout + first * LANES + threadIdx.x;
+  const uint4 *o = out + first * LANES + tid, *d = dout + first * LANES + tid;
   float2* stats = const_cast<float2*>(p.stats);
 #pragma unroll 4
-  for (int r = threadIdx.x / LANES; r < 128; r += STEP, o += 256, d += 256) {
+  for (int rb = 0; rb < rows; rb += STEP, o += THREADS, d += THREADS) {
+    const int r = rb + tid / LANES;
     uint4 x = make_uint4(0, 0, 0, 0), y = x;
     float l = 0.f;
     if (r < rows) {
@@ -1375,7 +1412,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const BwdParams p, 
     const float s = row_sum<LANES>(dot8<BF16>(x, y));
     float g = 0.f;
     if constexpr (!BF16) g = row_sum<LANES>(dot8<BF16>(y, y));
-    if (r < rows && threadIdx.x % LANES == 0) {
+    if (r < rows && tid % LANES == 0) {
       const float nl = fmaf(-1.4426950408889634f, l, BwdScale<BF16>::kPExp);
       stats[first + r] = make_float2(nl, -s);
       uint4 e = ext_columns<BF16>(nl * ext_mul, -s);
@@ -1389,56 +1426,62 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const BwdParams p, 
     }
   }
   if constexpr (!BF16) {
-    g_max = __reduce_max_sync(0xffffffffu, g_max);
-    d_max = __reduce_max_sync(0xffffffffu, d_max);
-    if (lane == 0) {
-      atomicMax(&code[0], g_max);
-      atomicMax(&code[1], d_max);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) *reinterpret_cast<int2*>(&p.range[first].x) = make_int2(code[0], code[1]);
+    g_max = largest(__reduce_max_sync(0xffffffffu, g_max), &code[0]);
+    d_max = largest(__reduce_max_sync(0xffffffffu, d_max), &code[1]);
+    if (tid == 0) *reinterpret_cast<int2*>(&p.range[first].x) = make_int2(g_max, d_max);
   }
 }
 
 // float16, packed: what range_by_sequence needs.  The first blocks find the code
-// of the largest |v| of each context, 128 rows of an entry each, and leave it at
+// of the largest |v| of each context, SLOTS slots of 128 rows each, and leave it at
 // the sequence that sees it (a shared context's at the head's first row; the
 // kernel before zeroed it).  The others gather the tiles' codes of a sequence and
-// head, a warp each.  Maxima of whole numbers do not depend on their order.
-template <int D>
+// head, a warp each; for v also those of the sequences before it.  Maxima of whole
+// numbers do not depend on their order.
+template <int D, int SLOTS>
 __global__ void __launch_bounds__(128) attn_bwd_range_kernel(const BwdParams p, const BwdRows vc, int context_blocks) {
   const int lane = threadIdx.x & 31;
   if ((int)blockIdx.x < context_blocks) {
-    __shared__ int code;
-    if (threadIdx.x == 0) code = 0;
-    __syncthreads();
-    const int h = blockIdx.x / p.cslots, slot = blockIdx.x % p.cslots;
+    constexpr int THREADS = 128 / SLOTS;
+    const long long i = (long long)blockIdx.x * SLOTS + threadIdx.x / THREADS;
+    const int h = (int)(i / p.cslots), slot = (int)(i % p.cslots);
+    if (h >= p.HK) return;
     const int c = find_slot_owner(p.cu_c, p.C, slot, lane);
     const int c0 = min(max(__ldg(p.cu_c + c), 0), p.Tc), c1 = min(max(__ldg(p.cu_c + c + 1), 0), p.Tc);
     const int t = slot - ((c0 >> 7) + c), r0 = c0 + t * 128, rows = t >= 0 ? min(c1 - r0, 128) : 0;
     int q0 = 0, q1 = 1;
     if (p.C > 1) packed_rows(p, c, q0, q1);
     if (rows <= 0 || q1 <= q0) return;  // (an entry that no query sees)
-    const int x = largest_norm_code<D, 128>(vc.data + h * vc.head + r0 * vc.row, vc.row, rows, &code);
-    if (threadIdx.x == 0) atomicMax(&p.range[(long long)h * p.T + q0].w, x);
+    const int x = largest_norm_code<D, THREADS>(vc.data + h * vc.head + r0 * vc.row, vc.row, rows, threadIdx.x % THREADS);
+    if (lane == 0) atomicMax(&p.range[(long long)h * p.T + q0].w, x);
     return;
   }
   const long long i = (long long)(blockIdx.x - context_blocks) * 4 + (threadIdx.x >> 5);  // query heads, then v's
   const int head = (int)(i / p.B), b = (int)(i % p.B);
   if (head >= p.H + p.HK) return;
   const bool is_v = head >= p.H;
-  int n;
-  int4* x = p.range + range_row(p, 0, is_v ? head - p.H : head, b, n);
-  int g = 0, d = 0;  // (v: its code in g)
-  for (int t = lane * 128; t < n; t += 32 * 128) {
-    g = max(g, is_v ? x[t].z : x[t].x);
-    if (!is_v) d = max(d, x[t].y);
+  int4* x = p.range + (long long)(is_v ? head - p.H : head) * p.T;
+  int s0, s1;
+  packed_rows(p, b, s0, s1);
+  if (s1 <= s0) return;
+  int g = 0, d = 0;  // (v: its code in g, that of all sequences up to it in d)
+  for (int r = s0 + lane * 128; r < s1; r += 32 * 128) {
+    g = max(g, (is_v ? x[r].z : x[r].x) & 255);  // (z may have been gathered already)
+    if (!is_v) d = max(d, x[r].y);
   }
   g = __reduce_max_sync(0xffffffffu, g);
+  if (is_v && p.causal) {
+    d = g;
+    for (int e = lane; e < b; e += 32) {
+      int e0, e1;
+      packed_rows(p, e, e0, e1);
+      for (int r = e0; r < e1; r += 128) d = max(d, x[r].z & 255);
+    }
+  }
   d = __reduce_max_sync(0xffffffffu, d);
-  if (lane != 0 || n <= 128) return;
-  if (is_v) x->z = g;
-  else *reinterpret_cast<int2*>(x) = make_int2(g, d);
+  if (lane != 0) return;
+  if (is_v) x[s0].z = g | d << 8;
+  else *reinterpret_cast<int2*>(x + s0) = make_int2(g, d);
 }
 
 }  // namespace fmlm
