@@ -9,6 +9,8 @@ in q, k and the norm's weights.
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd import forward_ad
 
@@ -37,6 +39,8 @@ class RotaryTable:
         if pairs not in _PAIRS:
             raise ValueError('pairs must be "half" or "interleaved"')
         if inv_freq is None:
+            if not 0.0 < float(base) < math.inf:
+                raise ValueError("base must be positive and finite")
             inv_freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
         if tuple(inv_freq.shape) != (rotary_dim // 2,):
             raise ValueError("inv_freq must have rotary_dim / 2 elements")
