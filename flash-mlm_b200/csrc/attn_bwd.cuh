@@ -58,8 +58,8 @@
 // Roles of a persistent CTA (one per SM): warps 0-15 do the element-wise work
 // (warp w: TMEM lanes 32 (w % 4) .., column quarter w / 4 of every score tile),
 // warp 16 loads tiles by TMA and decodes work items, warp 17 issues the MMAs,
-// warp 18 (KV) copies the streamed rows' extra columns, warp 19 (KV, float16)
-// finds dS's power of two.
+// warp 18 (KV) copies the streamed rows' extra columns, warps 18 (items of one
+// tile) and 19 (KV, float16) find dS's power of two.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -385,7 +385,7 @@ struct __align__(8) BwdBarriers {
   uint64_t sum_full;          // Q: every warp's part of delta is in shared memory
   uint64_t acc_full, acc_empty;
   uint64_t item_full[4], item_empty[4];
-  uint64_t mul_full[4];       // KV, float16: extra-column warp -> element-wise: the item's ds_mul
+  uint64_t mul_full[4];       // KV, float16: extra-column or power warp -> element-wise: the item's ds_mul
   int item_idx[4];
   uint32_t tmem_base;
   int abort_flag;
@@ -509,7 +509,7 @@ __device__ __forceinline__ uint8_t* ext_row(uint8_t* tile, int r, int h) {
 // The extra columns' units (A's constants): four columns of B1 for lse, three
 // of B2 for delta.  bfloat16 has float32's exponents, so three numbers of one
 // unit hold a value to 2^-27 of it.  float16 has not: its units fall by 2^11
-// or 2^12, the bits of one number.  lse, in units of q k^T, fits to 2^-36 of it
+// or 2^12, the bits of one number.  lse, in units of q k^T, fits to 2^-48 of it
 // or 2^-39, whichever is larger, up to 65504 * 2^15; delta to 2^-36 of it or
 // 2^-37, up to 65504 * 2^12.  What is larger saturates, and the KV pass says so.
 template <bool BF16>
@@ -1335,8 +1335,7 @@ __device__ __forceinline__ int largest_norm_code(const uint16_t* src, long long 
 // that follow.  Reads O and dO once (bound by HBM).  delta uses the 16-bit O that
 // the forward pass returned (what that costs: at the head of this file).
 // float16: also the rows' codes of |dO| and each tile's largest; the blocks behind
-// do the same for v's tiles.  A block takes SLOTS tile slots of 128 rows, one after the
-// other's heads: one where there are few, so that they spread over the GPU,
+// do the same for v's tiles.  A block takes SLOTS tile slots of 128 rows: one, or
 // eight (a warp each) where there are many of few rows (4096 sequences of 1 to 16
 // tokens, 8 heads: 26 us, one slot a block 103; 16 sequences of 512, 32 heads of
 // 128: one slot a block 27 us, eight 52).
